@@ -422,8 +422,11 @@ void spmm_msweep_kernel(const uint32_t* __restrict__ ent, const float* __restric
             // ONE monotonic counter per team: arrival = fetch-add, the barrier opens when the count reaches the next multiple of 32 (exactly 32
             // arrivals per barrier, so launches start on a multiple and nothing has to be reset; the last arriver is through after one L2
             // round trip, the others after their next poll).  Wrap-around: compared as a signed difference.
-            unsigned t = 1u;
-            asm volatile("s_atomic_add %0, %1, 0x0 glc\n\ts_waitcnt lgkmcnt(0)" : "+s"(t) : "s"(ctr) : "memory");
+            // Arrival and poll are one lane's vector memory operations (agent scope, as the census words).
+            unsigned t = 0u;
+            asm volatile("" ::: "memory");
+            if (lane == 0) t = ag_add(ctr, 1u);
+            t = (unsigned)__builtin_amdgcn_readfirstlane((int)t);
             if ((t & 31u) != 31u) {
                 const unsigned target = (t & ~31u) + 32u;
                 const unsigned long long tb = __builtin_amdgcn_s_memrealtime();
@@ -431,7 +434,8 @@ void spmm_msweep_kernel(const uint32_t* __restrict__ ent, const float* __restric
                 while (!open) {
                     __builtin_amdgcn_s_sleep(2);
                     unsigned v = 0u;
-                    asm volatile("s_atomic_add %0, %1, 0x0 glc\n\ts_waitcnt lgkmcnt(0)" : "+s"(v) : "s"(ctr) : "memory");
+                    if (lane == 0) v = ag_load(ctr);
+                    v = (unsigned)__builtin_amdgcn_readfirstlane((int)v);
                     open = (int)(v - target) >= 0;
                     if (!open && __builtin_amdgcn_s_memrealtime() - tb > (unsigned long long)tmo_ticks) break;
                 }
@@ -441,6 +445,7 @@ void spmm_msweep_kernel(const uint32_t* __restrict__ ent, const float* __restric
                     s_ctl[3] = 1u;
                 }
             }
+            asm volatile("" ::: "memory");
         }
         __syncthreads();
         return s_ctl[3] == 0u;
@@ -647,8 +652,9 @@ void spmm_msweep_kernel(const uint32_t* __restrict__ ent, const float* __restric
 
             const bool dependent = nhops > 1 && pass == passes - 1 && hop + 1 < nhops;   // the next hop gathers what this one stores
             if (use_barrier || dependent) {
-                // XCD barrier (no state to zero between launches: a captured launch replays as is).  Scalar atomics:
-                // they execute in the XCD's L2 and wait on lgkmcnt, not on the stores' vmcnt.  Between the hops of an entry the barrier
+                // XCD barrier (no state to zero between launches: a captured launch replays as is).  One lane per workgroup arrives and
+                // polls with vector atomics / loads at agent scope; the arrival's return waits for the wave's own stores as well (in-order
+                // vmcnt).  Between the hops of an entry the barrier
                 // orders this hop's stores (acknowledged by the L2: vmcnt(0)) before the next hop's gathers from the other CUs of the team --
                 // the team IS the set of workgroups on one XCC (census above), so counters and rows live in the one L2 they all use.  The
                 // census has seen all 256 workgroups resident; a barrier that still does not open within the time limit (a team mate died)

@@ -23,7 +23,7 @@ def is_hub(name):
 def main():
     with tempfile.TemporaryDirectory() as d:
         out = os.path.join(d, "k.s")
-        subprocess.run(["/opt/rocm/bin/hipcc", "-O3", "-std=c++17", "--offload-arch=gfx950", "-I" + os.path.join(ROOT, "include"), "-I" + os.path.join(PK, "csrc"),
+        subprocess.run(["/opt/rocm/bin/hipcc", "-O3", "-std=c++17", "--offload-arch=gfx950", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-I" + os.path.join(ROOT, "include"), "-I" + os.path.join(PK, "csrc"),
                         "-S", "--cuda-device-only", os.path.join(PK, "csrc", "gf_msweep.hip"), "-o", out], check=True, capture_output=True)
         txt = open(out).read()
     bad = nk = 0
