@@ -13,9 +13,10 @@ Layout mirrors the reference package so that call sites read the same:
 `install(reference_gml)` rebinds the reference's own symbols.
 """
 from .functional import EVGF_edges, LSIGF
+from .functional_seq import linear_recurrence
 from .gso import EdgePattern, SparseGSO
 
-__all__ = ["LSIGF", "EVGF_edges", "SparseGSO", "EdgePattern", "install"]
+__all__ = ["LSIGF", "EVGF_edges", "SparseGSO", "EdgePattern", "linear_recurrence", "install"]
 __version__ = "0.1.0"
 
 

@@ -14,6 +14,8 @@ if os.environ.get("GFHIP_EXPERIMENTS") == "1" and os.environ.get("GFHIP_LIB"):  
 
 GF_OK, GF_ERR_SHAPE = 0, -1
 GF_OP_FWD, GF_OP_BWD = 0, 1
+GF_F32, GF_BF16, GF_F16 = 0, 1, 2
+GF_GATE_N, GF_GATE_H, GF_GATE_B = 1, 2, 4
 
 _lib = None
 
@@ -70,6 +72,11 @@ _SIGNATURES = {
     "gf_nvgf_forward": (_c.c_int, [_c.POINTER(_vp), _i32, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _i32, _i32, _i32, _i32, _i32, _vp]),
     "gf_nvgf_backward": (_c.c_int, [_c.POINTER(_vp), _i32, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _i32, _i32, _i32, _i32, _i32, _vp]),
     "gf_nvgf_fold_taps": (_c.c_int, [_vp, _vp, _vp, _vp, _c.c_int64, _i32, _i32, _vp]),
+    "gf_recurrence_checkpoint_floats": (_sz, [_i32] * 7),
+    "gf_recurrence_workspace_bytes": (_sz, [_i32] * 8),
+    "gf_recurrence_forward": (_c.c_int, [_vp, _vp, _i32, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _i32, _i32, _i32, _i32, _i32, _vp]),
+    "gf_recurrence_backward": (_c.c_int, [_vp, _vp, _i32, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz,
+                                          _i32, _i32, _i32, _i32, _i32, _vp]),
     "gf_debug_msweep_trace": (_c.c_int, [_vp]),
     "gf_spmm_hop_kernel": (_c.c_int, [_vp, _i32, _i32, _i32]),
     "gf_debug_msweep_info": (_c.c_int, [_vp, _i32, _c.POINTER(_i32)]),

@@ -261,6 +261,30 @@ int gf_time_khop(const gf_plan* const* plans, int32_t E, int32_t op, float* Z, i
 int gf_time_spmm_hop(const gf_plan* plan, int32_t op, const float* X_in, float* X_out, int32_t B, int32_t W,
                      int32_t iters, void* stream, float* avg_ms);
 
+/* ---- sequence and output operators: element types and gates ------------------------------------------------------------------
+ * Tensors named "dtype" below hold fp32, bf16 or fp16 elements (void*); states, sums and statistics are fp32. */
+enum { GF_F32 = 0, GF_BF16 = 1, GF_F16 = 2 };
+/* a gate has shape [B|1, T, H|1, N|1], contiguous; the bits say which axes it has (none = one value per time step for all) */
+enum { GF_GATE_N = 1, GF_GATE_H = 2, GF_GATE_B = 4 };
+
+/* Gated linear recurrence  z_t = q_check_t z_{t-1} + q_hat_t u_t,  t = 1..T  (the recursion of GatedGRNN, graphML.py:1421-1462, with
+ * an identity B(S) and sigma; gates as q_hat / q_check there).  u, z [B, T, H, N] dtype; q_check, q_hat dtype (q_hat NULL = 1);
+ * z0 [B, H, N] fp32 (NULL = 0); lengths [B] int32 on the device (NULL = T; values are clamped to [0, T]): steps at or behind a sequence's
+ * length are not read, leave the state as it is and give z = 0.  zT [B, H, N] fp32 is the last state.
+ * checkpoints (gf_recurrence_checkpoint_floats, NULL = not kept): one fp32 state every few steps, what the backward pass recomputes the
+ * states from.  Products of q_check over a few hundred steps must stay finite in fp32.
+ * Tensors are aligned to four elements.  B >= 1, T >= 0, H N < 2^30. */
+size_t gf_recurrence_checkpoint_floats(int32_t B, int32_t T, int32_t H, int32_t N, int32_t kind_check, int32_t has_hat, int32_t kind_hat);
+size_t gf_recurrence_workspace_bytes(int32_t B, int32_t T, int32_t H, int32_t N, int32_t kind_check, int32_t has_hat, int32_t kind_hat, int32_t backward);
+int gf_recurrence_forward(const void* u, const void* q_check, int32_t kind_check, const void* q_hat, int32_t kind_hat, const float* z0,
+                          const int32_t* lengths, void* z, float* zT, float* checkpoints, void* workspace, size_t workspace_bytes,
+                          int32_t dtype, int32_t B, int32_t T, int32_t H, int32_t N, void* stream);
+/* dz [B, T, H, N] dtype and dzT [B, H, N] fp32 (each may be NULL = 0) -> du, dq_check, dq_hat (dtype, in the gates' shapes, summed over
+ * the axes a gate does not have in a fixed order), dz0 [B, H, N] fp32; NULL outputs are skipped. */
+int gf_recurrence_backward(const void* u, const void* q_check, int32_t kind_check, const void* q_hat, int32_t kind_hat, const int32_t* lengths,
+                           const float* checkpoints, const void* dz, const float* dzT, void* du, void* dq_check, void* dq_hat, float* dz0,
+                           void* workspace, size_t workspace_bytes, int32_t dtype, int32_t B, int32_t T, int32_t H, int32_t N, void* stream);
+
 /* ---- tuning / debugging knobs (no reference counterpart; results are identical for every setting):
  * "spmm_bt" (0 = heuristic | 1 | 2 | 4), "spmm_spw" (0 = default | 1 | 2 | 4 slices per wave), "spmm_generic" (0/1),
  * "spmm_algo" (0 = default: the MFMA source sweep (gf_msweep.hip) where it applies, else the SELL-8 wave kernel | 1 = CSR workgroup
