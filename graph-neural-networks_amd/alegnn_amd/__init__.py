@@ -13,10 +13,11 @@ Layout mirrors the reference package so that call sites read the same:
 `install(reference_gml)` rebinds the reference's own symbols.
 """
 from .functional import EVGF_edges, LSIGF
+from .functional_out import distill_top, token_log_probs
 from .functional_seq import linear_recurrence
 from .gso import EdgePattern, SparseGSO
 
-__all__ = ["LSIGF", "EVGF_edges", "SparseGSO", "EdgePattern", "linear_recurrence", "install"]
+__all__ = ["LSIGF", "EVGF_edges", "SparseGSO", "EdgePattern", "linear_recurrence", "token_log_probs", "distill_top", "install"]
 __version__ = "0.1.0"
 
 

@@ -77,6 +77,12 @@ _SIGNATURES = {
     "gf_recurrence_forward": (_c.c_int, [_vp, _vp, _i32, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _i32, _i32, _i32, _i32, _i32, _vp]),
     "gf_recurrence_backward": (_c.c_int, [_vp, _vp, _i32, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz,
                                           _i32, _i32, _i32, _i32, _i32, _vp]),
+    "gf_token_logp_workspace_bytes": (_sz, [_i64, _i32, _i32, _i32]),
+    "gf_token_logp_forward": (_c.c_int, [_vp, _i64, _vp, _c.c_float, _i64, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _sz, _i32, _i64, _i32, _vp]),
+    "gf_token_logp_backward": (_c.c_int, [_vp, _i64, _vp, _c.c_float, _i64, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _i32, _i64, _i32, _vp]),
+    "gf_distill_top_workspace_bytes": (_sz, [_i64, _i32, _i32, _i32]),
+    "gf_distill_top_forward": (_c.c_int, [_vp, _i64, _vp, _vp, _c.c_float, _i32, _vp, _vp, _vp, _vp, _sz, _i32, _i64, _i32, _i32, _vp]),
+    "gf_distill_top_backward": (_c.c_int, [_vp, _i64, _vp, _vp, _vp, _c.c_float, _i32, _vp, _vp, _i32, _i64, _i32, _i32, _vp]),
     "gf_debug_msweep_trace": (_c.c_int, [_vp]),
     "gf_spmm_hop_kernel": (_c.c_int, [_vp, _i32, _i32, _i32]),
     "gf_debug_msweep_info": (_c.c_int, [_vp, _i32, _c.POINTER(_i32)]),

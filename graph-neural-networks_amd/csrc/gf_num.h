@@ -37,3 +37,17 @@ template <typename D, int V> __device__ __forceinline__ void gf_store(D* __restr
 
 static inline size_t gf_dtype_bytes(int dtype) { return dtype == GF_F32 ? 4 : 2; }
 static inline bool gf_dtype_ok(int dtype) { return dtype == GF_F32 || dtype == GF_BF16 || dtype == GF_F16; }
+
+// the same at any element's address
+template <typename D, int V> struct __attribute__((packed, aligned(sizeof(D)))) gf_vec_any { D e[V]; };
+template <typename D, int V> __device__ __forceinline__ void gf_load_any(const D* __restrict__ p, float (&out)[V]) {
+    const gf_vec_any<D, V> r = *reinterpret_cast<const gf_vec_any<D, V>*>(p);
+#pragma unroll
+    for (int i = 0; i < V; ++i) out[i] = gf_to_f<D>(r.e[i]);
+}
+template <typename D, int V> __device__ __forceinline__ void gf_store_any(D* __restrict__ p, const float (&v)[V]) {
+    gf_vec_any<D, V> r;
+#pragma unroll
+    for (int i = 0; i < V; ++i) r.e[i] = gf_from_f<D>(v[i]);
+    *reinterpret_cast<gf_vec_any<D, V>*>(p) = r;
+}

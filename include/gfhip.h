@@ -285,6 +285,36 @@ int gf_recurrence_backward(const void* u, const void* q_check, int32_t kind_chec
                            const float* checkpoints, const void* dz, const float* dzT, void* du, void* dq_check, void* dq_hat, float* dz0,
                            void* workspace, size_t workspace_bytes, int32_t dtype, int32_t B, int32_t T, int32_t H, int32_t N, void* stream);
 
+/* Log probabilities of given tokens (classes, nodes) with entropy and best alternatives: the answers of a classifier (what evaluation.py:58-71 reduces to an
+ * error rate).  logits: R rows of V elements (dtype), row r at r * row_stride elements, unit stride inside a row; tokens [R] int64: the
+ * given output of each row; ignore_index marks a row without one (logp 0), any other token outside [0, V) gives NaN.
+ *   lp = log softmax(logits / temperature);  logp [R] = lp[token], entropy [R] = -sum p lp (NULL = not wanted), top_tokens / top_logp
+ *   [R, top]: the `top` largest logits of each row, largest first, equal ones in ascending index order (NaN counts as the largest).
+ * stats [R, 3] fp32 (row maximum, log of the sum, entropy): what the backward pass needs.  -inf marks an output that is ruled out
+ * (p = 0); a row of nothing else has logp = -inf, entropy 0 and gradient 0.  0 <= top <= min(V, 64).  No alignment is assumed. */
+size_t gf_token_logp_workspace_bytes(int64_t R, int32_t V, int32_t top, int32_t dtype);
+int gf_token_logp_forward(const void* logits, int64_t row_stride, const int64_t* tokens, float temperature, int64_t ignore_index, float* logp,
+                          float* entropy, float* top_logp, int64_t* top_tokens, int32_t top, float* stats, void* workspace, size_t workspace_bytes,
+                          int32_t dtype, int64_t R, int32_t V, void* stream);
+/* dlogp, dentropy [R], dtop [R, top] fp32 (each may be NULL = 0) -> dlogits [R, V] dtype, contiguous. */
+int gf_token_logp_backward(const void* logits, int64_t row_stride, const int64_t* tokens, float temperature, int64_t ignore_index, const float* stats,
+                           const int64_t* top_tokens, int32_t top, const float* dlogp, const float* dentropy, const float* dtop, void* dlogits,
+                           int32_t dtype, int64_t R, int32_t V, void* stream);
+
+/* Distillation from a teacher's K best outputs: loss [R] fp32 of the student's logits (R rows of V, dtype, as above) against the teacher's
+ * indices [R, K] int64 and values [R, K] fp32; entries with an index outside [0, V) are padding.  q = softmax(logits / temperature).
+ *   tail = 0: p = softmax(values / temperature) over the row's entries;  loss = sum_k p_k (log p_k - log q[i_k])
+ *   tail = 1: values are log probabilities, p_k = exp(values_k), what is left to one is one further outcome "none of these":
+ *             loss = sum_k p_k (log p_k - log q[i_k]) + p_r (log p_r - log q_r),  q_r = sum of q over the outputs not named
+ * A row without entries has loss 0 and gradient 0; an index named twice counts as two entries.  1 <= K <= 64.
+ * stats [R, 3] and probs [R, K] fp32: what the backward pass needs. */
+size_t gf_distill_top_workspace_bytes(int64_t R, int32_t V, int32_t K, int32_t dtype);
+int gf_distill_top_forward(const void* logits, int64_t row_stride, const int64_t* indices, const float* values, float temperature, int32_t tail,
+                           float* loss, float* stats, float* probs, void* workspace, size_t workspace_bytes, int32_t dtype, int64_t R, int32_t V,
+                           int32_t K, void* stream);
+int gf_distill_top_backward(const void* logits, int64_t row_stride, const int64_t* indices, const float* probs, const float* stats, float temperature,
+                            int32_t tail, const float* dloss, void* dlogits, int32_t dtype, int64_t R, int32_t V, int32_t K, void* stream);
+
 /* ---- tuning / debugging knobs (no reference counterpart; results are identical for every setting):
  * "spmm_bt" (0 = heuristic | 1 | 2 | 4), "spmm_spw" (0 = default | 1 | 2 | 4 slices per wave), "spmm_generic" (0/1),
  * "spmm_algo" (0 = default: the MFMA source sweep (gf_msweep.hip) where it applies, else the SELL-8 wave kernel | 1 = CSR workgroup
