@@ -11,24 +11,24 @@ from __future__ import annotations
 import math
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .functional import _ptr
-from .functional_seq import _DTYPES, _require_cuda
+from .functional_seq import _DTYPES, _FLOATS, _on, _once, _require_cuda, _stream
 
 TOP_MAX = 64
+_I64 = (torch.int64,)
 
 
 def _rows(who, logits, dim):
     """(rows as [R, V] with unit stride inside a row, leading shape): a view where the strides allow it, a copy otherwise."""
     assert logits.dim() >= 1 and -logits.dim() <= dim < logits.dim(), f"{who}: dim {dim} of logits with shape {tuple(logits.shape)}"
-    _require_cuda(who, "logits", logits, tuple(_DTYPES))
+    _require_cuda(who, "logits", logits, _FLOATS)
     if dim % logits.dim() != logits.dim() - 1:
         logits = logits.movedim(dim, -1)
     V = logits.shape[-1]
     assert V > 0, f"{who}: logits have shape {tuple(logits.shape)}: no outputs to choose from"
-    x = logits.reshape(-1, V)
+    x = logits if logits.dim() == 2 else logits.reshape(-1, V)
     if V > 1 and x.stride(1) != 1:
         x = x.contiguous()
     return x, logits.shape[:-1]
@@ -49,20 +49,38 @@ def _same_device(who, name, t, x):
 def _tokens_forward(x, tokens, top, temperature, ignore_index, entropy, keep):
     L = _lib.lib()
     R, V = x.shape
-    dev = x.device
-    with torch.cuda.device(dev):
+    dev, dt = x.device, _DTYPES[x.dtype]
+    with _on(dev):
         logp = torch.empty(R, dtype=torch.float32, device=dev)
         ent = torch.empty(R, dtype=torch.float32, device=dev) if entropy else None
         tl = torch.empty((R, top), dtype=torch.float32, device=dev) if top else None
         ti = torch.empty((R, top), dtype=torch.int64, device=dev) if top else None
         stats = torch.empty((R, 3), dtype=torch.float32, device=dev) if keep else None
         if R:
-            nb = L.gf_token_logp_workspace_bytes(R, V, top, _DTYPES[x.dtype])
-            ws = torch.empty(nb // 4, dtype=torch.float32, device=dev)
+            nb = L.gf_token_logp_workspace_bytes(R, V, top, dt)
+            ws = torch.empty(nb, dtype=torch.uint8, device=dev)
             _lib.check(L.gf_token_logp_forward(x.data_ptr(), x.stride(0), tokens.data_ptr(), temperature, ignore_index, logp.data_ptr(), _ptr(ent),
-                                               _ptr(tl), _ptr(ti), top, _ptr(stats), ws.data_ptr(), nb, _DTYPES[x.dtype], R, V,
-                                               torch.cuda.current_stream().cuda_stream), "gf_token_logp_forward")
+                                               _ptr(tl), _ptr(ti), top, _ptr(stats), ws.data_ptr(), nb, dt, R, V, _stream(dev)),
+                       "gf_token_logp_forward")
     return logp, ent, tl, ti, stats
+
+
+def _tokens_backward(ctx, dlogp, dent, dtop, _):
+    L = _lib.lib()
+    x, tokens, stats, ti = ctx.saved_tensors
+    top, temperature, ignore_index = ctx.args
+    R, V = x.shape
+    dev = x.device
+    if dlogp is None and dent is None and dtop is None:
+        return (None,) * 6
+    dlogp, dent, dtop = (None if g is None else g.contiguous() for g in (dlogp, dent, dtop))
+    with _on(dev):
+        dx = torch.empty((R, V), dtype=x.dtype, device=dev)
+        if R:
+            _lib.check(L.gf_token_logp_backward(x.data_ptr(), x.stride(0), tokens.data_ptr(), temperature, ignore_index, stats.data_ptr(), _ptr(ti),
+                                                top, _ptr(dlogp), _ptr(dent), _ptr(dtop), dx.data_ptr(), _DTYPES[x.dtype], R, V, _stream(dev)),
+                       "gf_token_logp_backward")
+    return dx, None, None, None, None, None
 
 
 class _TokenLogProbsFunction(torch.autograd.Function):
@@ -79,22 +97,8 @@ class _TokenLogProbsFunction(torch.autograd.Function):
         return logp, ent, tl, ti
 
     @staticmethod
-    @once_differentiable
-    def backward(ctx, dlogp, dent, dtop, _):
-        L = _lib.lib()
-        x, tokens, stats, ti = ctx.saved_tensors
-        top, temperature, ignore_index = ctx.args
-        R, V = x.shape
-        if dlogp is None and dent is None and dtop is None:
-            return (None,) * 6
-        dlogp, dent, dtop = (None if g is None else g.contiguous() for g in (dlogp, dent, dtop))
-        with torch.cuda.device(x.device):
-            dx = torch.empty((R, V), dtype=x.dtype, device=x.device)
-            if R:
-                _lib.check(L.gf_token_logp_backward(x.data_ptr(), x.stride(0), tokens.data_ptr(), temperature, ignore_index, stats.data_ptr(), _ptr(ti),
-                                                    top, _ptr(dlogp), _ptr(dent), _ptr(dtop), dx.data_ptr(), _DTYPES[x.dtype], R, V,
-                                                    torch.cuda.current_stream().cuda_stream), "gf_token_logp_backward")
-        return dx, None, None, None, None, None
+    def backward(ctx, *grads):
+        return _once(_tokens_backward, ctx, *grads)
 
 
 def token_log_probs(logits, tokens, top=0, temperature=1.0, ignore_index=-100, entropy=True, dim=-1):
@@ -113,7 +117,7 @@ def token_log_probs(logits, tokens, top=0, temperature=1.0, ignore_index=-100, e
     top = int(top)
     assert 0 <= top <= min(x.shape[1], TOP_MAX), f"{who}: top={top} for {x.shape[1]} outputs (want 0..min(V, {TOP_MAX}))"
     assert tokens.shape == lead, f"{who}: tokens have shape {tuple(tokens.shape)}, logits {tuple(logits.shape)} with the classes along {dim}"
-    _require_cuda(who, "tokens", tokens, (torch.int64,))
+    _require_cuda(who, "tokens", tokens, _I64)
     _same_device(who, "tokens", tokens, x)
     tokens = tokens.reshape(-1).contiguous()
     args = (x, tokens, top, temperature, int(ignore_index), bool(entropy))
@@ -130,18 +134,33 @@ def token_log_probs(logits, tokens, top=0, temperature=1.0, ignore_index=-100, e
 def _distill_forward(x, indices, values, temperature, tail):
     L = _lib.lib()
     (R, V), K = x.shape, indices.shape[1]
-    dev = x.device
-    with torch.cuda.device(dev):
+    dev, dt = x.device, _DTYPES[x.dtype]
+    with _on(dev):
         loss = torch.empty(R, dtype=torch.float32, device=dev)
-        stats = torch.empty((R, 3), dtype=torch.float32, device=dev)
-        probs = torch.empty((R, K), dtype=torch.float32, device=dev)
+        kept = torch.empty(R * (3 + K), dtype=torch.float32, device=dev)            # stats [R, 3], then the named outputs' coefficients [R, K]
         if R:
-            nb = L.gf_distill_top_workspace_bytes(R, V, K, _DTYPES[x.dtype])
-            ws = torch.empty(nb // 4, dtype=torch.float32, device=dev)
+            nb = L.gf_distill_top_workspace_bytes(R, V, K, dt)
+            ws = torch.empty(nb, dtype=torch.uint8, device=dev)
+            at = kept.data_ptr()
             _lib.check(L.gf_distill_top_forward(x.data_ptr(), x.stride(0), indices.data_ptr(), values.data_ptr(), temperature, tail, loss.data_ptr(),
-                                                stats.data_ptr(), probs.data_ptr(), ws.data_ptr(), nb, _DTYPES[x.dtype], R, V, K,
-                                                torch.cuda.current_stream().cuda_stream), "gf_distill_top_forward")
-    return loss, stats, probs
+                                                at, at + 12 * R, ws.data_ptr(), nb, dt, R, V, K, _stream(dev)), "gf_distill_top_forward")
+    return loss, kept
+
+
+def _distill_backward(ctx, dloss):
+    L = _lib.lib()
+    x, indices, kept = ctx.saved_tensors
+    temperature, tail = ctx.args
+    (R, V), K = x.shape, indices.shape[1]
+    dev = x.device
+    dloss = dloss.contiguous()
+    with _on(dev):
+        dx = torch.empty((R, V), dtype=x.dtype, device=dev)
+        if R:
+            at = kept.data_ptr()
+            _lib.check(L.gf_distill_top_backward(x.data_ptr(), x.stride(0), indices.data_ptr(), at + 12 * R, at, temperature, tail, dloss.data_ptr(),
+                                                 dx.data_ptr(), _DTYPES[x.dtype], R, V, K, _stream(dev)), "gf_distill_top_backward")
+    return dx, None, None, None, None
 
 
 class _DistillTopFunction(torch.autograd.Function):
@@ -149,26 +168,14 @@ class _DistillTopFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, indices, values, temperature, tail):
-        loss, stats, probs = _distill_forward(x, indices, values, temperature, tail)
+        loss, kept = _distill_forward(x, indices, values, temperature, tail)
         ctx.args = (temperature, tail)
-        ctx.save_for_backward(x, indices, stats, probs)
+        ctx.save_for_backward(x, indices, kept)
         return loss
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dloss):
-        L = _lib.lib()
-        x, indices, stats, probs = ctx.saved_tensors
-        temperature, tail = ctx.args
-        (R, V), K = x.shape, indices.shape[1]
-        dloss = dloss.contiguous()
-        with torch.cuda.device(x.device):
-            dx = torch.empty((R, V), dtype=x.dtype, device=x.device)
-            if R:
-                _lib.check(L.gf_distill_top_backward(x.data_ptr(), x.stride(0), indices.data_ptr(), probs.data_ptr(), stats.data_ptr(), temperature,
-                                                     tail, dloss.data_ptr(), dx.data_ptr(), _DTYPES[x.dtype], R, V, K,
-                                                     torch.cuda.current_stream().cuda_stream), "gf_distill_top_backward")
-        return dx, None, None, None, None
+        return _once(_distill_backward, ctx, dloss)
 
 
 def distill_top(logits, indices, values, temperature=1.0, tail=False, dim=-1):
@@ -190,15 +197,17 @@ def distill_top(logits, indices, values, temperature=1.0, tail=False, dim=-1):
     assert 1 <= K <= TOP_MAX, f"{who}: indices have shape {tuple(indices.shape)} (want [..., K] with 1 <= K <= {TOP_MAX})"
     assert indices.shape == (*lead, K) and values.shape == indices.shape, (
         f"{who}: indices {tuple(indices.shape)} and values {tuple(values.shape)} for logits {tuple(logits.shape)} with the classes along {dim}")
-    _require_cuda(who, "indices", indices, (torch.int64,))
-    _require_cuda(who, "values", values, tuple(_DTYPES))
+    _require_cuda(who, "indices", indices, _I64)
+    _require_cuda(who, "values", values, _FLOATS)
     _same_device(who, "indices", indices, x)
     _same_device(who, "values", values, x)
     if values.requires_grad and torch.is_grad_enabled():
         raise NotImplementedError("distill_top: values.requires_grad is not supported (the teacher's outputs are constants); detach them")
-    args = (x, indices.reshape(-1, K).contiguous(), values.reshape(-1, K).float().contiguous(), temperature, int(bool(tail)))
+    if indices.dim() != 2:
+        indices, values = indices.reshape(-1, K), values.reshape(-1, K)
+    args = (x, indices.contiguous(), values.float().contiguous(), temperature, int(bool(tail)))
     if torch.is_grad_enabled() and x.requires_grad:
         loss = _DistillTopFunction.apply(*args)
     else:
         loss = _distill_forward(*args)[0]
-    return loss.view(lead)
+    return loss if len(lead) == 1 else loss.view(lead)

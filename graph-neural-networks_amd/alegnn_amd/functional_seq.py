@@ -7,6 +7,8 @@ one filter per step; the gates are GatedGRNN's q_hat / q_check (time, node) and,
 """
 from __future__ import annotations
 
+import contextlib
+
 import torch
 from torch.autograd.function import once_differentiable
 
@@ -14,6 +16,22 @@ from . import _lib
 from .functional import _ptr
 
 _DTYPES = {torch.float32: _lib.GF_F32, torch.bfloat16: _lib.GF_BF16, torch.float16: _lib.GF_F16}
+_FLOATS = tuple(_DTYPES)
+_F32 = (torch.float32,)
+_I32 = (torch.int32,)
+_HERE = contextlib.nullcontext()
+
+# The calls below are a few microseconds of GPU work at the reference's own sizes, so the host side counts: device and stream are asked for
+# without building torch's Python objects, scratch and statistics share one allocation, and double backward is refused only when asked for.
+
+
+def _on(dev):
+    """The tensors' device as the current one (nothing to do in the usual case)."""
+    return _HERE if torch._C._cuda_getDevice() == dev.index else torch.cuda.device(dev)
+
+
+def _stream(dev):
+    return torch._C._cuda_getCurrentRawStream(dev.index)
 
 
 def _require_cuda(who, name, t, dtypes):
@@ -49,7 +67,7 @@ def _forward(u, qc, qh, z0, lengths, keep):
     kc = _gate_kind(qc, u.shape, "q_check")
     kh = 0 if qh is None else _gate_kind(qh, u.shape, "q_hat")
     hat = 0 if qh is None else 1
-    with torch.cuda.device(dev):
+    with _on(dev):
         z = torch.empty((B, T, H, N), dtype=u.dtype, device=dev)
         zT = torch.empty((B, H, N), dtype=torch.float32, device=dev)
         if u.numel() == 0 and B * H * N == 0:
@@ -60,9 +78,39 @@ def _forward(u, qc, qh, z0, lengths, keep):
         nb = L.gf_recurrence_workspace_bytes(B, T, H, N, kc, hat, kh, 0)
         ws = torch.empty(nb // 4, dtype=torch.float32, device=dev) if nb else None
         _lib.check(L.gf_recurrence_forward(u.data_ptr(), qc.data_ptr(), kc, _ptr(qh), kh, _ptr(z0), _ptr(lengths), z.data_ptr(), zT.data_ptr(),
-                                           _ptr(ckpt), _ptr(ws), nb, _DTYPES[u.dtype], B, T, H, N, torch.cuda.current_stream().cuda_stream),
+                                           _ptr(ckpt), _ptr(ws), nb, _DTYPES[u.dtype], B, T, H, N, _stream(dev)),
                    "gf_recurrence_forward")
     return z, zT, ckpt, (kc, kh, hat)
+
+
+def _once(f, ctx, *grads):
+    """f(ctx, *grads); under create_graph the result refuses to be differentiated again."""
+    return once_differentiable(f)(ctx, *grads) if torch.is_grad_enabled() else f(ctx, *grads)
+
+
+def _recurrence_backward(ctx, dz, dzT):
+    L = _lib.lib()
+    u, qc, qh, lengths, ckpt = ctx.saved_tensors
+    kc, kh, hat = ctx.kinds
+    B, T, H, N = u.shape
+    dev = u.device
+    need_u, need_c, need_h, need_0 = ctx.needs_input_grad[:4]
+    if dz is None and dzT is None:
+        return None, None, None, None, None
+    dz, dzT = _dense(dz), _dense(dzT)
+    with _on(dev):
+        du = torch.empty_like(u) if need_u else None
+        dqc = torch.empty_like(qc) if need_c else None
+        dqh = torch.empty_like(qh) if need_h else None
+        dz0 = torch.empty((B, H, N), dtype=torch.float32, device=dev) if need_0 else None
+        if B * H * N == 0:
+            return du, None if dqc is None else dqc.zero_(), None if dqh is None else dqh.zero_(), dz0, None
+        nb = L.gf_recurrence_workspace_bytes(B, T, H, N, kc, hat, kh, 1)
+        ws = torch.empty(nb // 4, dtype=torch.float32, device=dev) if nb else None
+        _lib.check(L.gf_recurrence_backward(u.data_ptr(), qc.data_ptr(), kc, _ptr(qh), kh, _ptr(lengths), _ptr(ckpt), _ptr(dz), _ptr(dzT),
+                                            _ptr(du), _ptr(dqc), _ptr(dqh), _ptr(dz0), _ptr(ws), nb, _DTYPES[u.dtype], B, T, H, N,
+                                            _stream(dev)), "gf_recurrence_backward")
+    return du, dqc, dqh, dz0, None
 
 
 class _LinearRecurrenceFunction(torch.autograd.Function):
@@ -77,30 +125,8 @@ class _LinearRecurrenceFunction(torch.autograd.Function):
         return z, zT
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dz, dzT):
-        L = _lib.lib()
-        u, qc, qh, lengths, ckpt = ctx.saved_tensors
-        kc, kh, hat = ctx.kinds
-        B, T, H, N = u.shape
-        dev = u.device
-        need_u, need_c, need_h, need_0 = ctx.needs_input_grad[:4]
-        if dz is None and dzT is None:
-            return None, None, None, None, None
-        dz, dzT = _dense(dz), _dense(dzT)
-        with torch.cuda.device(dev):
-            du = torch.empty_like(u) if need_u else None
-            dqc = torch.empty_like(qc) if need_c else None
-            dqh = torch.empty_like(qh) if need_h else None
-            dz0 = torch.empty((B, H, N), dtype=torch.float32, device=dev) if need_0 else None
-            if B * H * N == 0:
-                return du, None if dqc is None else dqc.zero_(), None if dqh is None else dqh.zero_(), dz0, None
-            nb = L.gf_recurrence_workspace_bytes(B, T, H, N, kc, hat, kh, 1)
-            ws = torch.empty(nb // 4, dtype=torch.float32, device=dev) if nb else None
-            _lib.check(L.gf_recurrence_backward(u.data_ptr(), qc.data_ptr(), kc, _ptr(qh), kh, _ptr(lengths), _ptr(ckpt), _ptr(dz), _ptr(dzT),
-                                                _ptr(du), _ptr(dqc), _ptr(dqh), _ptr(dz0), _ptr(ws), nb, _DTYPES[u.dtype], B, T, H, N,
-                                                torch.cuda.current_stream().cuda_stream), "gf_recurrence_backward")
-        return du, dqc, dqh, dz0, None
+        return _once(_recurrence_backward, ctx, dz, dzT)
 
 
 def linear_recurrence(u, q_check, q_hat=None, z0=None, lengths=None):
@@ -114,7 +140,7 @@ def linear_recurrence(u, q_check, q_hat=None, z0=None, lengths=None):
     over a few hundred steps must stay finite (gates in [-1, 1] always do).  Differentiable (once) in u, q_check, q_hat and z0."""
     who = "linear_recurrence"
     assert u.dim() == 4, f"{who}: u has shape {tuple(u.shape)}, want [B, T, H, N]"
-    _require_cuda(who, "u", u, tuple(_DTYPES))
+    _require_cuda(who, "u", u, _FLOATS)
     for name, q in (("q_check", q_check), ("q_hat", q_hat)):
         if q is not None:
             _gate_kind(q, u.shape, name)
@@ -122,11 +148,11 @@ def linear_recurrence(u, q_check, q_hat=None, z0=None, lengths=None):
             assert q.device == u.device, f"{who}: {name} is on {q.device}, u on {u.device}"
     if z0 is not None:
         assert tuple(z0.shape) == (u.shape[0], u.shape[2], u.shape[3]), f"{who}: z0 has shape {tuple(z0.shape)} for u {tuple(u.shape)}"
-        _require_cuda(who, "z0", z0, (torch.float32,))
+        _require_cuda(who, "z0", z0, _F32)
         assert z0.device == u.device, f"{who}: z0 is on {z0.device}, u on {u.device}"
     if lengths is not None:
         assert tuple(lengths.shape) == (u.shape[0],), f"{who}: lengths has shape {tuple(lengths.shape)}, want [{u.shape[0]}]"
-        _require_cuda(who, "lengths", lengths, (torch.int32,))
+        _require_cuda(who, "lengths", lengths, _I32)
         assert lengths.device == u.device, f"{who}: lengths is on {lengths.device}, u on {u.device}"
         lengths = lengths.contiguous()
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (u, q_check, q_hat, z0)):
