@@ -22,8 +22,10 @@
 
 namespace {
 
-constexpr int kL = 8;              // steps per thread and slab: 8 independent loads per array in flight
-constexpr int kMaxSplit = 64;
+constexpr int kL = 4;              // steps per thread and slab.  8 steps need twice the registers and lose: backward of 32 x 257 x 53824 bf16 in 1.32 ms
+                                   // against 1.69 ms, of 65537 x 808 in 301 us against 416 us (both before the straight-line loads)
+constexpr int kGW = 4;             // time groups of a wave: 4 (rows of 16 lanes) against 8: 0.89 / 1.02 ms, against 2 with 8 steps: 0.89 / 0.97 ms
+constexpr int kMaxSplit = 128;     // splits of a long time axis: 128 / 64 / 256 give 307 / 344 / 323 us for 65537 x 808 bf16, forward and backward
 
 struct Gate {                      // a gate of shape [B|1, T, H|1, N|1]: element (b, t, h, n) at b sb + t st + channel offset
     const void* p;
@@ -40,16 +42,32 @@ struct Dims {
     int32_t nck;                   // checkpoints per sequence
 };
 
+// The loads of a slab are straight-line code (addresses clamped to the last live step, values replaced afterwards): all of them are in
+// flight before the first one is waited for.  A gate without the node axis has one value for the thread's V channels (V > 1 only where they
+// share the feature); it is spread after the other loads have been issued.
 template <typename D, int V>
-__device__ __forceinline__ void load_gate(const Gate& g, int64_t base, int coff, int t, float (&out)[V]) {
-    const D* p = static_cast<const D*>(g.p) + base + (int64_t)t * g.st + coff;
-    if (g.kind & GF_GATE_N) {
-        gf_load<D, V>(p, out);
-    } else {                       // one value for the thread's V channels (V > 1 only where they share the feature)
-        const float v = gf_to_f<D>(*p);
+__device__ __forceinline__ void load_gate(const Gate& g, int64_t at, const int (&t)[kL], gf_vec<D, V> (&raw)[kL]) {
+    const D* p = static_cast<const D*>(g.p) + at;
+    if (V > 1 && (g.kind & GF_GATE_N)) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) out[i] = v;
+        for (int l = 0; l < kL; ++l) raw[l] = *reinterpret_cast<const gf_vec<D, V>*>(p + (int64_t)t[l] * g.st);
+    } else {
+#pragma unroll
+        for (int l = 0; l < kL; ++l) raw[l].e[0] = p[(int64_t)t[l] * g.st];
     }
+}
+template <typename D, int V> __device__ __forceinline__ void spread_gate(const Gate& g, gf_vec<D, V> (&raw)[kL]) {
+    if (V > 1 && !(g.kind & GF_GATE_N)) {
+#pragma unroll
+        for (int l = 0; l < kL; ++l)
+#pragma unroll
+            for (int i = 1; i < V; ++i) raw[l].e[i] = raw[l].e[0];
+    }
+}
+template <typename D, int V>
+__device__ __forceinline__ void load_rows(const D* __restrict__ p, int64_t C, const int (&t)[kL], gf_vec<D, V> (&raw)[kL]) {
+#pragma unroll
+    for (int l = 0; l < kL; ++l) raw[l] = *reinterpret_cast<const gf_vec<D, V>*>(p + t[l] * C);
 }
 __device__ __forceinline__ int gate_coff(const Gate& g, int c, int N) {
     if (g.kind == (GF_GATE_H | GF_GATE_N)) return c;
@@ -148,6 +166,28 @@ __device__ __forceinline__ void join(const float (&A)[V], const float (&S)[V], f
     }
 }
 
+// composition of the splits [s0, s1) of the thread's channels, shared out over the time groups (walked forwards or backwards)
+template <int V, int WT, int GW, bool FWD>
+__device__ __forceinline__ void join_splits(const float* __restrict__ agg, int64_t all, int64_t chan, int s0, int s1, const Place<V, WT, GW>& p,
+                                            float (&At)[V], float (&St)[V], float* lds) {
+    constexpr int TG = WT * GW;
+    const int q = (s1 - s0 + TG - 1) / TG, lo = min(s1, s0 + p.tg * q), hi = min(s1, lo + q);
+    float A[V], S[V], Ae[V], Se[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) A[i] = 1.f, S[i] = 0.f;
+#pragma unroll 4
+    for (int k = lo; k < hi; ++k) {
+        const float* g = agg + 2 * (int64_t)(FWD ? k : lo + hi - 1 - k) * all + chan;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const float ak = g[i];
+            S[i] = fmaf(ak, S[i], g[all + i]);
+            A[i] *= ak;
+        }
+    }
+    join<V, WT, GW, FWD>(A, S, Ae, Se, At, St, p.lane, p.wave, lds);
+}
+
 // ---- forward -------------------------------------------------------------------------------------------------------------
 // AGG: the first kernel of a split run -- no outputs but each split's (A, h)
 template <typename D, int V, int WT, int GW, bool AGG>
@@ -161,46 +201,67 @@ __global__ __launch_bounds__(64 * (WT == 1 ? 4 : WT)) void recur_fwd_kernel(cons
     if (AGG && p.split == d.splits - 1) return;                 // nothing starts behind the last split
     int len = d.T;
     if (lengths) len = min(max(lengths[p.b], 0), d.T);
-    const int64_t ub = (int64_t)p.b * d.T * d.C + p.c, chan = (int64_t)p.b * d.C + p.c, all = (int64_t)d.B * d.C;
-    const int64_t cb = p.b * gc.sb, hb = p.b * gh.sb;
-    const int coff = gate_coff(gc, p.c, d.N), hoff = gate_coff(gh, p.c, d.N);
+    const int pc = p.on ? p.c : d.C - V;                        // lanes behind the last channel read its values and store nothing
+    const int64_t ub = (int64_t)p.b * d.T * d.C + pc, chan = (int64_t)p.b * d.C + pc, all = (int64_t)d.B * d.C;
+    const int64_t cb = p.b * gc.sb + gate_coff(gc, pc, d.N), hb = p.b * gh.sb + gate_coff(gh, pc, d.N);
     float carry[V], Asum[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) carry[i] = 0.f, Asum[i] = 1.f;
-    if (!AGG && p.on) {
+    if (!AGG) {
         if (z0) {
 #pragma unroll
             for (int i = 0; i < V; ++i) carry[i] = z0[chan + i];
         }
-        for (int s = 0; s < p.split; ++s) {
+    }
+    if (!AGG && p.split > 0) {                                  // (uniform) the splits before this one
+        float At[V], St[V];
+        join_splits<V, WT, GW, true>(agg, all, chan, 0, p.split, p, At, St, s_join[WT == 1 ? 0 : 1]);
 #pragma unroll
-            for (int i = 0; i < V; ++i) carry[i] = fmaf(agg[(2 * (int64_t)s) * all + chan + i], carry[i], agg[(2 * (int64_t)s + 1) * all + chan + i]);
-        }
+        for (int i = 0; i < V; ++i) carry[i] = fmaf(At[i], carry[i], St[i]);
     }
     const int tbeg = p.split * d.split_len, tend = min(d.T, tbeg + d.split_len);
+    const int live_end = min(tend, len);
+    gf_vec<D, V> ra[kL], rb[kL], rq[kL];
+    auto fetch = [&](int ts) {
+        int t[kL];
+#pragma unroll
+        for (int l = 0; l < kL; ++l) t[l] = min(ts + p.tg * kL + l, len - 1);
+        load_rows<D, V>(u + ub, d.C, t, rb);
+        load_gate<D, V>(gc, cb, t, ra);
+        if (gh.p) load_gate<D, V>(gh, hb, t, rq);
+    };
+    if (tbeg < live_end) fetch(tbeg);
     int flip = 0;
     for (int ts = tbeg; ts < tend; ts += P::SLAB, flip ^= 1) {
         const int t0 = ts + p.tg * kL;
-        float a[kL][V], b[kL][V], A[V], S[V];
-#pragma unroll
-        for (int l = 0; l < kL; ++l) {
-#pragma unroll
-            for (int i = 0; i < V; ++i) a[l][i] = 1.f, b[l][i] = 0.f;
-            if (p.on && t0 + l < len) {
-                load_gate<D, V>(gc, cb, coff, t0 + l, a[l]);
-                gf_load<D, V>(u + ub + (int64_t)(t0 + l) * d.C, b[l]);
+        if (ts >= len) {                                        // (uniform) behind the sequence: the state stays, the output is zero
+            if (!AGG && p.on) {
+                const float zero[V] = {};
+                for (int l = 0; l < kL; ++l)
+                    if (t0 + l < d.T) gf_store<D, V>(z + ub + (int64_t)(t0 + l) * d.C, zero);
             }
+            continue;
         }
+        float a[kL][V], b[kL][V], A[V], S[V];
+        spread_gate<D, V>(gc, ra);
+#pragma unroll
+        for (int l = 0; l < kL; ++l)
+#pragma unroll
+            for (int i = 0; i < V; ++i) a[l][i] = gf_to_f<D>(ra[l].e[i]), b[l][i] = gf_to_f<D>(rb[l].e[i]);
         if (gh.p) {
+            spread_gate<D, V>(gh, rq);
 #pragma unroll
-            for (int l = 0; l < kL; ++l) {
-                if (p.on && t0 + l < len) {
-                    float q[V];
-                    load_gate<D, V>(gh, hb, hoff, t0 + l, q);
+            for (int l = 0; l < kL; ++l)
 #pragma unroll
-                    for (int i = 0; i < V; ++i) b[l][i] *= q[i];
-                }
-            }
+                for (int i = 0; i < V; ++i) b[l][i] *= gf_to_f<D>(rq[l].e[i]);
+        }
+        if (ts + P::SLAB < live_end) fetch(ts + P::SLAB);       // (into the registers just read: the next slab loads while this one is joined)
+        if (ts + P::SLAB > len) {                               // (uniform) the sequence ends in this slab
+#pragma unroll
+            for (int l = 0; l < kL; ++l)
+#pragma unroll
+                for (int i = 0; i < V; ++i)
+                    if (t0 + l >= len) a[l][i] = 1.f, b[l][i] = 0.f;
         }
 #pragma unroll
         for (int i = 0; i < V; ++i) A[i] = 1.f, S[i] = 0.f;
@@ -221,7 +282,7 @@ __global__ __launch_bounds__(64 * (WT == 1 ? 4 : WT)) void recur_fwd_kernel(cons
         }
         if (!AGG && p.on) {
             if (ckpt && t0 < d.T && t0 % d.every == 0) {
-                float* k = ckpt + ((int64_t)p.b * d.nck + t0 / d.every) * d.C + p.c;
+                float* k = ckpt + ((int64_t)p.b * d.nck + t0 / d.every) * d.C + pc;
 #pragma unroll
                 for (int i = 0; i < V; ++i) k[i] = h[i];
             }
@@ -270,7 +331,7 @@ __device__ __forceinline__ void put_gate(const GateOut& g, const float (&v)[V], 
     } else if (g.mode == kOutTime) {
         float s = 0.f;
 #pragma unroll
-        for (int i = 0; i < V; ++i) s += v[i];
+        for (int i = 0; i < V; ++i) s += on ? v[i] : 0.f;
 #pragma unroll
         for (int off2 = 1; off2 < CX; off2 <<= 1) s += __shfl_xor(s, off2);
         if (live && lane % CX == 0) static_cast<float*>(g.p)[toff] = s;
@@ -288,43 +349,89 @@ __global__ __launch_bounds__(64 * (WT == 1 ? 4 : WT)) void recur_bwd_kernel(cons
     if (AGG && p.split == 0) return;
     int len = d.T;
     if (lengths) len = min(max(lengths[p.b], 0), d.T);
-    const int64_t ub = (int64_t)p.b * d.T * d.C + p.c, chan = (int64_t)p.b * d.C + p.c, all = (int64_t)d.B * d.C;
-    const int64_t cb = p.b * gc.sb, hb = p.b * gh.sb;
-    const int coff = gate_coff(gc, p.c, d.N), hoff = gate_coff(gh, p.c, d.N);
+    const int pc = p.on ? p.c : d.C - V;
+    const int64_t ub = (int64_t)p.b * d.T * d.C + pc, chan = (int64_t)p.b * d.C + pc, all = (int64_t)d.B * d.C;
+    const int64_t cb = p.b * gc.sb + gate_coff(gc, pc, d.N), hb = p.b * gh.sb + gate_coff(gh, pc, d.N);
     // sums over a wave's channels (time gates): one row of [B, T] per wave column
     const int64_t cols = (int64_t)(blockIdx.x % (unsigned)d.chunks) * (WT == 1 ? P::NW : 1) + (WT == 1 ? p.wave : 0);
     const int64_t tbase = (cols * d.B + p.b) * d.T;
     float carry[V], Asum[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) carry[i] = 0.f, Asum[i] = 1.f;
-    if (!AGG && p.on) {
+    if (!AGG) {
         if (dzT) {
 #pragma unroll
             for (int i = 0; i < V; ++i) carry[i] = dzT[chan + i];
         }
-        for (int s = d.splits - 1; s > p.split; --s) {
+    }
+    if (!AGG && p.split + 1 < d.splits) {                       // (uniform) the splits behind this one
+        float At[V], St[V];
+        join_splits<V, WT, GW, false>(agg, all, chan, p.split + 1, d.splits, p, At, St, s_join[WT == 1 ? 0 : 2]);
 #pragma unroll
-            for (int i = 0; i < V; ++i) carry[i] = fmaf(agg[(2 * (int64_t)s) * all + chan + i], carry[i], agg[(2 * (int64_t)s + 1) * all + chan + i]);
-        }
+        for (int i = 0; i < V; ++i) carry[i] = fmaf(At[i], carry[i], St[i]);
     }
     const int tbeg = p.split * d.split_len, tend = min(d.T, tbeg + d.split_len);
     const int slabs = tend > tbeg ? (tend - tbeg + P::SLAB - 1) / P::SLAB : 0;
+    gf_vec<D, V> ra[kL], rx[kL], rq[kL], rg[kL];
+    auto fetch = [&](int ts) {
+        int t[kL];
+#pragma unroll
+        for (int l = 0; l < kL; ++l) t[l] = min(ts + p.tg * kL + l, len - 1);
+        if (dz) load_rows<D, V>(dz + ub, d.C, t, rg);
+        load_gate<D, V>(gc, cb, t, ra);
+        if (!AGG) {
+            load_rows<D, V>(u + ub, d.C, t, rx);
+            if (gh.p) load_gate<D, V>(gh, hb, t, rq);
+        }
+    };
+    if (tbeg < min(tend, len)) fetch(tbeg + (min(tend, len) - tbeg - 1) / P::SLAB * P::SLAB);     // the last slab with a live step
     int flip = 0;
     for (int sl = slabs - 1; sl >= 0; --sl, flip ^= 2) {
         const int ts = tbeg + sl * P::SLAB, t0 = ts + p.tg * kL;
-        float a[kL][V], x[kL][V], q[kL][V], g[kL][V], A[V], R[V];
-#pragma unroll
-        for (int l = 0; l < kL; ++l) {
-#pragma unroll
-            for (int i = 0; i < V; ++i) a[l][i] = 1.f, x[l][i] = 0.f, q[l][i] = 1.f, g[l][i] = 0.f;
-            if (p.on && t0 + l < len) {
-                load_gate<D, V>(gc, cb, coff, t0 + l, a[l]);
-                if (dz) gf_load<D, V>(dz + ub + (int64_t)(t0 + l) * d.C, g[l]);
-                if (!AGG) {
-                    gf_load<D, V>(u + ub + (int64_t)(t0 + l) * d.C, x[l]);
-                    if (gh.p) load_gate<D, V>(gh, hb, hoff, t0 + l, q[l]);
+        if (ts >= len) {                                        // (uniform) behind the sequence: nothing flows, the gradients are zero
+            if (!AGG) {
+                const float zero[V] = {};
+                for (int l = 0; l < kL; ++l) {
+                    const int64_t off = ub + (int64_t)(t0 + l) * d.C;
+                    if (du && p.on && t0 + l < d.T) gf_store<D, V>(du + off, zero);
+                    if (oc.mode) put_gate<D, V, P::CX>(oc, zero, off, tbase + t0 + l, p.on, t0 + l < d.T, p.lane);
+                    if (oh.mode) put_gate<D, V, P::CX>(oh, zero, off, tbase + t0 + l, p.on, t0 + l < d.T, p.lane);
                 }
             }
+            continue;
+        }
+        const bool ends = ts + P::SLAB > len;                   // (uniform) the sequence ends in this slab
+        float a[kL][V], x[kL][V], q[kL][V], g[kL][V], A[V], R[V];
+        spread_gate<D, V>(gc, ra);
+#pragma unroll
+        for (int l = 0; l < kL; ++l)
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                a[l][i] = gf_to_f<D>(ra[l].e[i]);
+                g[l][i] = 0.f;
+                x[l][i] = AGG ? 0.f : gf_to_f<D>(rx[l].e[i]);
+                q[l][i] = 1.f;
+            }
+        if (dz) {
+#pragma unroll
+            for (int l = 0; l < kL; ++l)
+#pragma unroll
+                for (int i = 0; i < V; ++i) g[l][i] = gf_to_f<D>(rg[l].e[i]);
+        }
+        if (!AGG && gh.p) {
+            spread_gate<D, V>(gh, rq);
+#pragma unroll
+            for (int l = 0; l < kL; ++l)
+#pragma unroll
+                for (int i = 0; i < V; ++i) q[l][i] = gf_to_f<D>(rq[l].e[i]);
+        }
+        if (sl > 0) fetch(ts - P::SLAB);                        // (into the registers just read: the next slab loads while this one is joined)
+        if (ends) {
+#pragma unroll
+            for (int l = 0; l < kL; ++l)
+#pragma unroll
+                for (int i = 0; i < V; ++i)
+                    if (t0 + l >= len) a[l][i] = 1.f, x[l][i] = 0.f, q[l][i] = 1.f, g[l][i] = 0.f;
         }
 #pragma unroll
         for (int i = 0; i < V; ++i) A[i] = 1.f, R[i] = 0.f;
@@ -356,7 +463,7 @@ __global__ __launch_bounds__(64 * (WT == 1 ? 4 : WT)) void recur_bwd_kernel(cons
                 join<V, WT, GW, true>(A, S, Ae, Se, At, St, p.lane, p.wave, s_join[WT == 1 ? 0 : flip + 1]);
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
-                    const float start = p.on ? ckpt[((int64_t)p.b * d.nck + ts / d.every) * d.C + p.c + i] : 0.f;
+                    const float start = ckpt[((int64_t)p.b * d.nck + ts / d.every) * d.C + pc + i];
                     h[i] = fmaf(Ae[i], start, Se[i]);
                 }
 #pragma unroll
@@ -369,21 +476,26 @@ __global__ __launch_bounds__(64 * (WT == 1 ? 4 : WT)) void recur_bwd_kernel(cons
             }
 #pragma unroll
             for (int l = kL - 1; l >= 0; --l) {
-                const int t = t0 + l;
-                const bool live = t < len;
                 float o[V], oq[V], ox[V];
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
                     const float gt = g[l][i] + r[i];            // dL/dz_t
-                    o[i] = live ? gt * zp[l][i] : 0.f;
-                    oq[i] = live ? gt * x[l][i] : 0.f;
-                    ox[i] = live ? gt * q[l][i] : 0.f;
+                    o[i] = gt * zp[l][i];
+                    oq[i] = gt * x[l][i];
+                    ox[i] = gt * q[l][i];
                     r[i] = a[l][i] * gt;
                 }
-                const int64_t off = ub + (int64_t)t * d.C;
-                if (du && p.on && t < d.T) gf_store<D, V>(du + off, ox);
-                if (oc.mode) put_gate<D, V, P::CX>(oc, o, off, tbase + t, p.on, t < d.T, p.lane);
-                if (oh.mode) put_gate<D, V, P::CX>(oh, oq, off, tbase + t, p.on, t < d.T, p.lane);
+                bool in = true;
+                if (ends) {                                     // padded steps pass the state's gradient on and have none of their own
+                    in = t0 + l < d.T;
+#pragma unroll
+                    for (int i = 0; i < V; ++i)
+                        if (t0 + l >= len) o[i] = oq[i] = ox[i] = 0.f;
+                }
+                const int64_t off = ub + (int64_t)(t0 + l) * d.C;
+                if (du && p.on && in) gf_store<D, V>(du + off, ox);
+                if (oc.mode) put_gate<D, V, P::CX>(oc, o, off, tbase + t0 + l, p.on, in, p.lane);
+                if (oh.mode) put_gate<D, V, P::CX>(oh, oq, off, tbase + t0 + l, p.on, in, p.lane);
             }
         }
     }
@@ -404,34 +516,50 @@ __global__ __launch_bounds__(64 * (WT == 1 ? 4 : WT)) void recur_bwd_kernel(cons
 // Sum of the fp32 products [rows, T, inner, H, N] ... over the axes a gate does not have, in a fixed order: out[b, t, h, n] (gate shape).
 // src [nb, B, T, Hs, Ns] : nb partial rows; axes: nb always, B if !GF_GATE_B, Hs if !(kind & H), Ns if !(kind & N).
 // One wave per output element where the node axis is summed, one thread per element otherwise (coalesced over nodes).
+__device__ __forceinline__ float sum_strided(const float* __restrict__ p, int n, int64_t stride, float s) {   // in order, eight loads in flight
+    int i = 0;
+    for (; i + 8 <= n; i += 8) {
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = p[(i + e) * stride];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s += v[e];
+    }
+    for (; i < n; ++i) s += p[i * stride];
+    return s;
+}
+
 template <typename D>
 __global__ __launch_bounds__(256) void recur_fold_kernel(const float* __restrict__ src, D* __restrict__ out, int nb, int B, int T, int Hs, int Ns,
                                                          int kind, int64_t total) {
     const bool byN = !(kind & GF_GATE_N) && Ns > 1;
     const int Ho = (kind & GF_GATE_H) ? Hs : 1, No = (kind & GF_GATE_N) ? Ns : 1, Bo = (kind & GF_GATE_B) ? B : 1;
     const int lane = threadIdx.x & 63;
-    const int64_t stride = byN ? (int64_t)gridDim.x * 4 : (int64_t)gridDim.x * 256;
+    const int64_t stride = byN ? (int64_t)gridDim.x * 4 : (int64_t)gridDim.x * 256, row = (int64_t)Hs * Ns;
     for (int64_t o = byN ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : (int64_t)blockIdx.x * 256 + threadIdx.x; o < total; o += stride) {
         const int n = (int)(o % No);
         const int64_t o1 = o / No;
         const int h = (int)(o1 % Ho);
         const int64_t o2 = o1 / Ho;
         const int t = (int)(o2 % T), b = (int)(o2 / T);
+        const float* p = src + ((int64_t)b * T + t) * row + (int64_t)h * Ns + n;
+        const int hs = Ho == 1 ? Hs : 1, bs = Bo == 1 ? B : 1;
         float s = 0.f;
-        for (int k = 0; k < nb; ++k)
-            for (int bb = (Bo == 1 ? 0 : b); bb < (Bo == 1 ? B : b + 1); ++bb)
-                for (int hh = (Ho == 1 ? 0 : h); hh < (Ho == 1 ? Hs : h + 1); ++hh) {
-                    const float* row = src + ((((int64_t)k * B + bb) * T + t) * Hs + hh) * Ns;
-                    if (byN)
-                        for (int m = lane; m < Ns; m += 64) s += row[m];
-                    else
-                        s += row[n];
-                }
         if (byN) {
+            for (int k = 0; k < nb * bs; ++k)                   // (nb > 1 only with Hs = Ns = 1)
+                for (int hh = 0; hh < hs; ++hh)
+                    for (int m = lane; m < Ns; m += 64) s += p[(int64_t)k * T * row + (int64_t)hh * Ns + m];
 #pragma unroll
             for (int off = 1; off < 64; off <<= 1) s += __shfl_xor(s, off);
             if (lane == 0) out[o] = gf_from_f<D>(s);
         } else {
+            if (hs > 1) {
+                for (int bb = 0; bb < bs; ++bb) s = sum_strided(p + (int64_t)bb * T * row, hs, Ns, s);
+            } else if (bs > 1) {
+                s = sum_strided(p, nb * bs, T * row, s);        // (partial rows of all sequences: [nb][B] is one axis)
+            } else {
+                s = sum_strided(p, nb, (int64_t)B * T * row, s);
+            }
             out[o] = gf_from_f<D>(s);
         }
     }
@@ -442,22 +570,23 @@ struct Shape {                     // what the kernels are chosen by: a function
     int V, WT, GW, slab, splits, split_len;
 };
 
-Shape choose(int B, int T, int64_t C, int N, int kinds, bool aligned4) {
+Shape choose(int B, int T, int64_t C, int N, int kinds) {
     Shape s;
     const bool within = kinds != 0;                             // some gate is shared along one of the two channel axes
-    s.V = (aligned4 && C % 4 == 0 && (!within || N % 4 == 0)) ? 4 : 1;
+    const int64_t by = within ? N : C;                          // (C is a multiple of N)
+    s.V = by % 4 == 0 ? 4 : by % 2 == 0 ? 2 : 1;
     const int64_t lanes = (int64_t)B * ((C + s.V - 1) / s.V);
     const int need = (T + kL - 1) / kL;                         // time groups that have work
     // enough threads to keep the memory busy (128k with 8 vector loads each), no more groups than there is time
     s.WT = 1, s.GW = 1;
-    if (need > 1) s.GW = 8;
+    if (need > 1) s.GW = kGW;
     if (need > 8 && lanes * 8 < 131072) s.WT = 4;
     s.slab = s.WT * s.GW * kL;
     const int64_t blocks = (int64_t)B * ((C + (int64_t)(s.WT == 1 ? 4 : 1) * (64 / s.GW) * s.V - 1) / ((int64_t)(s.WT == 1 ? 4 : 1) * (64 / s.GW) * s.V));
     const int slabs = (T + s.slab - 1) / s.slab;
     s.splits = 1;
     if (blocks < 256 && slabs >= 8) {                           // fewer workgroups than compute units and a long way to walk
-        int64_t want = (1024 + blocks - 1) / blocks;
+        int64_t want = (2048 + blocks - 1) / blocks;
         if (want > slabs / 4) want = slabs / 4;
         if (want > kMaxSplit) want = kMaxSplit;
         s.splits = want < 1 ? 1 : (int)want;
@@ -507,16 +636,16 @@ Dims make_dims(const Shape& s, int B, int T, int H, int N) {
     return d;
 }
 
+template <int V, typename F>
+int by_time(const Shape& s, F&& f) {
+    using std::integral_constant;
+    if (s.GW == 1) return f(integral_constant<int, V>(), integral_constant<int, 1>(), integral_constant<int, 1>());
+    if (s.WT == 1) return f(integral_constant<int, V>(), integral_constant<int, 1>(), integral_constant<int, kGW>());
+    return f(integral_constant<int, V>(), integral_constant<int, 4>(), integral_constant<int, kGW>());
+}
 template <typename F>
 int by_shape(const Shape& s, F&& f) {
-    if (s.V == 4) {
-        if (s.GW == 1) return f(std::integral_constant<int, 4>(), std::integral_constant<int, 1>(), std::integral_constant<int, 1>());
-        if (s.WT == 1) return f(std::integral_constant<int, 4>(), std::integral_constant<int, 1>(), std::integral_constant<int, 8>());
-        return f(std::integral_constant<int, 4>(), std::integral_constant<int, 4>(), std::integral_constant<int, 8>());
-    }
-    if (s.GW == 1) return f(std::integral_constant<int, 1>(), std::integral_constant<int, 1>(), std::integral_constant<int, 1>());
-    if (s.WT == 1) return f(std::integral_constant<int, 1>(), std::integral_constant<int, 1>(), std::integral_constant<int, 8>());
-    return f(std::integral_constant<int, 1>(), std::integral_constant<int, 4>(), std::integral_constant<int, 8>());
+    return s.V == 4 ? by_time<4>(s, f) : s.V == 2 ? by_time<2>(s, f) : by_time<1>(s, f);
 }
 
 int wave_columns(const Dims& d, const Shape& s) { return d.chunks * (s.WT == 1 ? 4 : 1); }
@@ -597,7 +726,7 @@ int backward_t(const Shape& s, const Dims& d, const void* u, Gate gc, Gate gh, c
 
 // the kernels' shape may not depend on pointers (forward and backward see different ones): V = 4 needs every tensor 4-element aligned,
 // which the callers below check and refuse otherwise
-Shape shape_of(int B, int T, int H, int N, int kc, bool has_h, int kh) { return choose(B, T, (int64_t)H * N, N, kind_bits(kc, has_h, kh), true); }
+Shape shape_of(int B, int T, int H, int N, int kc, bool has_h, int kh) { return choose(B, T, (int64_t)H * N, N, kind_bits(kc, has_h, kh)); }
 
 }  // namespace
 
