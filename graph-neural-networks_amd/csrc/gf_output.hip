@@ -21,6 +21,7 @@ namespace {
 
 constexpr int kThr = 256;
 constexpr int kTopMax = 64;
+constexpr int kMaxNV = 4;          // 16-byte groups per thread and tile: 4 / 8 / 2 take 162 / 189 / 177 us for 4096 x 50001 bf16 with 8 alternatives
 constexpr int kCand = 1024;        // candidates that are ranked in LDS; more (heavy ties) take the extraction loop
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -34,15 +35,52 @@ __device__ __forceinline__ unsigned ord32(float x) {            // order of floa
 __device__ __forceinline__ float unord32(unsigned o) { return __uint_as_float(o ^ ((o >> 31) ? 0x80000000u : 0xffffffffu)); }
 __device__ __forceinline__ u64 make_key(float x, int64_t j) { return ((u64)ord32(x) << 32) | (unsigned)~(unsigned)j; }
 
-__device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
-    return v;
+// reductions over the wave by lane shifts inside the vector unit (no LDS traffic); every lane gets the result.  Fixed order.
+template <int CTRL, int ROWS> __device__ __forceinline__ float dpp(float old, float v) {
+    return __uint_as_float(__builtin_amdgcn_update_dpp(__float_as_uint(old), __float_as_uint(v), CTRL, ROWS, 0xf, false));
 }
-template <typename T> __device__ __forceinline__ T wave_sum(T v) {
+__device__ __forceinline__ float last_lane(float v) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), 63)); }
+__device__ __forceinline__ float wave_max(float v) {
+    const float n = -INFINITY;
+    v = fmaxf(v, dpp<0x111, 0xf>(n, v));                        // rows of 16: shifted by 1, 2, 4, 8
+    v = fmaxf(v, dpp<0x112, 0xf>(n, v));
+    v = fmaxf(v, dpp<0x114, 0xf>(n, v));
+    v = fmaxf(v, dpp<0x118, 0xf>(n, v));
+    v = fmaxf(v, dpp<0x142, 0xa>(n, v));                        // last lane of a row to the next row, rows 1 and 3
+    v = fmaxf(v, dpp<0x143, 0xc>(n, v));                        // lane 31 to rows 2 and 3
+    return last_lane(v);
+}
+__device__ __forceinline__ float wave_sum(float v) {
+    v += dpp<0x111, 0xf>(0.f, v);
+    v += dpp<0x112, 0xf>(0.f, v);
+    v += dpp<0x114, 0xf>(0.f, v);
+    v += dpp<0x118, 0xf>(0.f, v);
+    v += dpp<0x142, 0xa>(0.f, v);
+    v += dpp<0x143, 0xc>(0.f, v);
+    return last_lane(v);
+}
+__device__ __forceinline__ double wave_sum(double v) {
 #pragma unroll
     for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
     return v;
+}
+__device__ __forceinline__ double lane_value(double v, int k) {  // lane k's value (k uniform)
+    return __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(v), k), __builtin_amdgcn_readlane(__double2loint(v), k));
+}
+__device__ __forceinline__ float exp2_fast(float y) { return __builtin_amdgcn_exp2f(y); }   // one instruction; results below 2^-126 are zero
+
+// how many of the n keys are larger than `key`, eight LDS reads in flight
+__device__ __forceinline__ int rank_of(const u64* keys, int n, u64 key) {
+    int rank = 0, q = 0;
+    for (; q + 8 <= n; q += 8) {
+        u64 k[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) k[e] = keys[q + e];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) rank += k[e] > key;
+    }
+    for (; q < n; ++q) rank += keys[q] > key;
+    return rank;
 }
 
 // A row's elements as 16-byte groups: group g holds elements g VE .. g VE + VE.  Rows of odd length start at any element: the group loads and stores
@@ -72,36 +110,79 @@ struct Parts {                     // per (row, tile): maximum, sums, and the ti
     u64* keys;
 };
 
-// k-th largest of the wave's 64 values (as ordered unsigned), by bits from the top; 16-bit types have no more than 16 significant ones
-template <int BITS> __device__ __forceinline__ unsigned kth_of_wave(unsigned v, int k) {
+// Lower bound of the k-th largest of the wave's 64 values (as ordered unsigned): its upper 16 bits, found bit by bit -- exact for bf16, and for the
+// other types a few values more pass (half the steps of an exact search).
+__device__ __forceinline__ unsigned kth_of_wave(unsigned v, int k) {
     unsigned thr = 0;
 #pragma unroll
-    for (int b = 31; b >= 32 - BITS; --b) {
+    for (int b = 31; b >= 16; --b) {
         const unsigned c = thr | (1u << b);
         if (__popcll(__ballot(v >= c)) >= k) thr = c;
     }
     return thr;
 }
 
+struct TokenOut {                  // what a row of token_log_probs is answered with
+    const int64_t* tokens;
+    int64_t ignore;
+    float *logp, *entropy, *top_logp;
+    int64_t* top_tokens;
+    float* stats;
+};
+// one thread: the row's statistics (maximum M, sum S, weighted sum T in natural units)
+template <typename D>
+__device__ __forceinline__ void answer_row(const TokenOut& o, int64_t r, const D* row, int V, float c, float M, float S, float T, float& ls) {
+    const bool empty = M == -INFINITY && S == 0.f;              // nothing but ruled-out outputs
+    ls = empty ? 0.f : logf(S);
+    const float H = empty ? 0.f : ls - T / S;
+    const int64_t y = o.tokens[r];
+    float lp = 0.f;
+    if (y != o.ignore) lp = (y < 0 || y >= V) ? NAN : empty ? -INFINITY : (gf_to_f<D>(row[y]) - M) * c - ls;
+    o.logp[r] = lp;
+    if (o.entropy) o.entropy[r] = H;
+    if (o.stats) o.stats[r * 3] = M, o.stats[r * 3 + 1] = ls, o.stats[r * 3 + 2] = H;
+}
+__device__ __forceinline__ void answer_top(const TokenOut& o, int64_t at, u64 key, float c, float M, float ls) {
+    const unsigned v = (unsigned)(key >> 32);
+    const float x = v == 0xfffffffeu ? NAN : unord32(v);
+    o.top_tokens[at] = (unsigned)~(unsigned)key;
+    o.top_logp[at] = (M == -INFINITY && ls == 0.f) ? -INFINITY : (x - M) * c - ls;
+}
+
 // ---- tile statistics (and best keys) -----------------------------------------------------------------------------------
-// MASK: the outputs named by indices[row][0..K) are left out
-template <typename D, int NV, bool TOP, bool MASK>
-__global__ __launch_bounds__(kThr) void tile_kernel(const D* __restrict__ logits, int64_t row_stride, int V, int tiles, float c2, int top,
-                                                    const int64_t* __restrict__ indices, int K, Parts out) {
+// TOP: the tile's best keys too; ENT: the weighted sum t; MASK: the outputs named by indices[row][0..K) are left out; ONE: a tile is a whole row and
+// answered here (tokens).  Each wave has a maximum of its own, so the sums need no workgroup barrier; the four waves join at the end.
+// The exponent is the difference first, then the scale (one fma of c2 x - c2 m overflows on masks of the type's lowest value).
+template <typename D, int NV, bool TOP, bool ENT, bool MASK, bool ONE>
+__global__ __launch_bounds__(kThr) void tile_kernel(const D* __restrict__ logits, int64_t row_stride, int V, int tiles, float c, int top,
+                                                    const int64_t* __restrict__ indices, int K, Parts out, TokenOut ans) {
     constexpr int VE = Row<D>::VE, TE = NV * kThr * VE;
-    __shared__ float s_m[4], s_s[4], s_t[4];
+    __shared__ float s_m[4], s_s[4], s_t[4], s_row[2];
     __shared__ unsigned s_thr[8];
     __shared__ int s_n;
     __shared__ u64 s_cand[TOP ? kCand : 1];
     __shared__ unsigned s_bits[MASK ? TE / 32 : 1];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int64_t r = blockIdx.x / (unsigned)tiles;
-    const int tile = (int)(blockIdx.x % (unsigned)tiles);
+    const int64_t r = ONE ? blockIdx.x : blockIdx.x / (unsigned)tiles;
+    const int tile = ONE ? 0 : (int)(blockIdx.x % (unsigned)tiles);
     const Row<D> row(logits + r * row_stride, V);
     const int64_t g0 = (int64_t)tile * NV * kThr;
     float x[NV][VE];
+    if (row.first(g0 + NV * kThr) <= V) {                       // (uniform) a tile inside the row: plain loads
+        gf_vec_any<D, VE> raw[NV];
 #pragma unroll
-    for (int v = 0; v < NV; ++v) row.load(g0 + v * kThr + tid, x[v], -INFINITY);
+        for (int v = 0; v < NV; ++v) raw[v] = *reinterpret_cast<const gf_vec_any<D, VE>*>(row.p + row.first(g0 + v * kThr + tid));
+#pragma unroll
+        for (int v = 0; v < NV; ++v)
+#pragma unroll
+            for (int e = 0; e < VE; ++e) x[v][e] = gf_to_f<D>(raw[v].e[e]);
+    } else {
+#pragma unroll
+        for (int v = 0; v < NV; ++v) row.load(g0 + v * kThr + tid, x[v], -INFINITY);
+    }
+    if constexpr (TOP) {
+        if (tid == 0) s_n = 0;
+    }
     if constexpr (MASK) {
         for (int i = tid; i < TE / 32; i += kThr) s_bits[i] = 0u;
         __syncthreads();
@@ -113,10 +194,12 @@ __global__ __launch_bounds__(kThr) void tile_kernel(const D* __restrict__ logits
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
             const int q = (v * kThr + tid) * VE;
-            const unsigned w = s_bits[q >> 5] >> (q & 31);
+            const unsigned w = (s_bits[q >> 5] >> (q & 31)) & ((1u << VE) - 1u);
+            if (w) {
 #pragma unroll
-            for (int e = 0; e < VE; ++e)
-                if (w >> e & 1u) x[v][e] = -INFINITY;
+                for (int e = 0; e < VE; ++e)
+                    if (w >> e & 1u) x[v][e] = -INFINITY;
+            }
         }
     }
     float tm = -INFINITY, vm[NV];
@@ -128,73 +211,96 @@ __global__ __launch_bounds__(kThr) void tile_kernel(const D* __restrict__ logits
         tm = fmaxf(tm, vm[v]);
     }
     const float wm = wave_max(tm);
-    if (lane == 0) s_m[wave] = wm;
     if constexpr (TOP) {
-        constexpr int BITS = sizeof(D) == 2 && std::is_same<D, gf_bf16>::value ? 16 : 32;
         const unsigned o = ord32(tm);
-        const unsigned a = kth_of_wave<BITS>(o, (top + 3) / 4), b = kth_of_wave<BITS>(o, top);
+        const unsigned a = kth_of_wave(o, (top + 3) / 4), b = kth_of_wave(o, top);
         if (lane == 0) s_thr[wave] = a, s_thr[4 + wave] = b;
-        if (tid == 0) s_n = 0;
     }
-    __syncthreads();
-    const float m = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
-    const float ref = m == -INFINITY ? 0.f : m;                 // a tile with nothing in it: all exponentials are zero
+    const float c2 = c * kLog2e, ref = wm == -INFINITY ? 0.f : wm;         // a wave with nothing in it: all exponentials are zero
     float s = 0.f, t = 0.f;
 #pragma unroll
     for (int v = 0; v < NV; ++v)
 #pragma unroll
         for (int e = 0; e < VE; ++e) {
             const float y = (x[v][e] - ref) * c2;               // base-2 exponent
-            const float p = exp2f(y);
+            const float p = exp2_fast(y);
             s += p;
-            t = fmaf(p, fmaxf(y, -3e38f), t);                   // p = 0 where y = -inf
+            if (ENT) t = fmaf(p, fmaxf(y, -3e38f), t);          // p = 0 where y = -inf
         }
     s = wave_sum(s);
-    t = wave_sum(t);
-    if (lane == 0) s_s[wave] = s, s_t[wave] = t;
+    if (ENT) t = wave_sum(t) * kLn2;
+    if (lane == 0) {
+        s_m[wave] = wm;
+        s_s[wave] = s;
+        s_t[wave] = t;
+    }
     __syncthreads();
-    s = (s_s[0] + s_s[1]) + (s_s[2] + s_s[3]);
-    t = (s_t[0] + s_t[1]) + (s_t[2] + s_t[3]);
+    float m = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
+    s = t = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        const float sw = s_s[w], mw = s_m[w];
+        if (mw == -INFINITY && sw == 0.f) continue;
+        const float y = (mw - m) * c, f = exp2_fast(y * kLog2e);
+        s = fmaf(sw, f, s);
+        if (ENT && f > 0.f) t = fmaf(fmaf(sw, y, s_t[w]), f, t);
+        if (f != f) s = t = f;
+    }
     const int64_t at = r * tiles + tile;
+    float ls = 0.f;
     if (tid == 0) {
-        out.m[at] = m;
-        out.s[at] = s;
-        out.t[at] = t * kLn2;
+        if constexpr (ONE) {
+            answer_row<D>(ans, r, row.p, V, c, m, s, t, ls);
+            s_row[0] = ls;
+        } else {
+            out.m[at] = m;
+            out.s[at] = s;
+            if (ENT) out.t[at] = t;
+        }
     }
     if constexpr (TOP) {
-        u64* keys = out.keys + at * top;
-        const int64_t jend = V;
+        u64* keys = ONE ? nullptr : out.keys + at * top;
+        auto put = [&](int k, u64 key) {
+            if constexpr (ONE) answer_top(ans, r * top + k, key, c, m, s_row[0]);
+            else keys[k] = key;
+        };
         bool ranked = false;
-        if (s == s) {                                           // no NaN in the tile: the maxima above are the values' own order
+        int n = 0;
+        const bool plain = s == s;                              // no NaN in the tile: the maxima above are the values' own order
+        if (plain) {
             unsigned ua = s_thr[0], ub = s_thr[4];
 #pragma unroll
             for (int w = 1; w < 4; ++w) ua = min(ua, s_thr[w]), ub = max(ub, s_thr[4 + w]);
             const unsigned u = max(ua, ub);
             const float thr = u < 0x00800000u ? -INFINITY : unord32(u);   // (bits below the ordered -inf = negative NaNs)
+            if (tm >= thr) {
 #pragma unroll
-            for (int v = 0; v < NV; ++v) {
-                if (vm[v] >= thr) {
-                    const int64_t j0 = row.first(g0 + v * kThr + tid);
+                for (int v = 0; v < NV; ++v) {
+                    if (vm[v] >= thr) {
+                        const int64_t j0 = row.first(g0 + v * kThr + tid);
 #pragma unroll
-                    for (int e = 0; e < VE; ++e) {
-                        if (x[v][e] >= thr && j0 + e < jend) {
-                            const int at2 = atomicAdd(&s_n, 1);
-                            if (at2 < kCand) s_cand[at2] = make_key(x[v][e], j0 + e);
+                        for (int e = 0; e < VE; ++e) {
+                            if (x[v][e] >= thr && j0 + e < V) {
+                                const int k = atomicAdd(&s_n, 1);
+                                if (k < kCand) s_cand[k] = make_key(x[v][e], j0 + e);
+                            }
                         }
                     }
                 }
             }
-            __syncthreads();
-            const int n = s_n;
+        }
+        __syncthreads();
+        if (plain) {
+            n = s_n;
             ranked = n <= kCand;
             if (ranked) {
                 for (int i = tid; i < n; i += kThr) {
                     const u64 key = s_cand[i];
-                    int rank = 0;
-                    for (int q = 0; q < n; ++q) rank += s_cand[q] > key;
-                    if (rank < top) keys[rank] = key;
+                    const int rank = rank_of(s_cand, n, key);
+                    if (rank < top) put(rank, key);
                 }
-                for (int i = n + tid; i < top; i += kThr) keys[i] = 0ull;
+                if constexpr (!ONE)
+                    for (int i = n + tid; i < top; i += kThr) keys[i] = 0ull;
             }
         }
         if (!ranked) {                                          // (uniform) heavy ties or NaN: extract the largest key below the last one, `top` times
@@ -206,7 +312,7 @@ __global__ __launch_bounds__(kThr) void tile_kernel(const D* __restrict__ logits
                     const int64_t j0 = row.first(g0 + v * kThr + tid);
 #pragma unroll
                     for (int e = 0; e < VE; ++e) {
-                        if (j0 + e < jend) {
+                        if (j0 + e < V) {
                             const u64 key = make_key(x[v][e], j0 + e);
                             if (key < last && key > best) best = key;
                         }
@@ -223,7 +329,7 @@ __global__ __launch_bounds__(kThr) void tile_kernel(const D* __restrict__ logits
                 best = s_cand[0];
 #pragma unroll
                 for (int w = 1; w < 4; ++w) best = s_cand[w] > best ? s_cand[w] : best;
-                if (tid == 0) keys[k] = best;
+                if (tid == 0) put(k, best);
                 last = best;                                    // 0 once the tile is used up: nothing is below it
             }
         }
@@ -231,7 +337,7 @@ __global__ __launch_bounds__(kThr) void tile_kernel(const D* __restrict__ logits
 }
 
 // the tiles' statistics of a row, joined (every lane of the wave gets them): maximum, sum, weighted sum
-__device__ __forceinline__ void join_tiles(const Parts& in, int64_t r, int tiles, float c, int lane, float& M, float& S, float& Tw) {
+__device__ __forceinline__ void join_tiles(const Parts& in, int64_t r, int tiles, float c, int lane, bool ent, float& M, float& S, float& Tw) {
     float m = -INFINITY;
     for (int i = lane; i < tiles; i += 64) m = fmaxf(m, in.m[r * tiles + i]);
     M = wave_max(m);
@@ -239,9 +345,9 @@ __device__ __forceinline__ void join_tiles(const Parts& in, int64_t r, int tiles
     for (int i = lane; i < tiles; i += 64) {
         const float mi = in.m[r * tiles + i], si = in.s[r * tiles + i];
         if (mi == -INFINITY && si == 0.f) continue;             // nothing in this tile
-        const float y = (mi - M) * c, w = exp2f(y * kLog2e);
+        const float y = (mi - M) * c, w = exp2_fast(y * kLog2e);
         s = fmaf(si, w, s);
-        if (w > 0.f) t = fmaf(fmaf(si, y, in.t[r * tiles + i]), w, t);
+        if (ent && w > 0.f) t = fmaf(fmaf(si, y, in.t[r * tiles + i]), w, t);
         if (w != w) t = w;
     }
     S = wave_sum(s);
@@ -250,59 +356,62 @@ __device__ __forceinline__ void join_tiles(const Parts& in, int64_t r, int tiles
 
 // ---- tokens: join the tiles of a row, answer --------------------------------------------------------------------------------
 template <typename D>
-__global__ __launch_bounds__(kThr) void token_finish_kernel(const D* __restrict__ logits, int64_t row_stride, const int64_t* __restrict__ tokens, float c,
-                                                            int64_t ignore_index, Parts in, int tiles, int V, int top, float* __restrict__ logp,
-                                                            float* __restrict__ entropy, float* __restrict__ top_logp, int64_t* __restrict__ top_tokens,
-                                                            float* __restrict__ stats) {
+__global__ __launch_bounds__(kThr) void token_finish_kernel(const D* __restrict__ logits, int64_t row_stride, float c, Parts in, int tiles, int V, int top,
+                                                            TokenOut ans) {
+    constexpr int kPer = 8;                                     // keys per thread and piece
     __shared__ float s_row[2];
-    __shared__ u64 s_key[2048 + kTopMax], s_best[kTopMax];
-    const int tid = threadIdx.x, lane = tid & 63;
+    __shared__ u64 s_cand[kPer * kThr + kTopMax], s_best[kTopMax];
+    __shared__ unsigned s_thr[8];
+    __shared__ int s_n;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int64_t r = blockIdx.x;
     if (tid < 64) {
-        float M, S, Tw;
-        join_tiles(in, r, tiles, c, lane, M, S, Tw);
+        float M, S, Tw, ls;
+        join_tiles(in, r, tiles, c, lane, true, M, S, Tw);
         if (lane == 0) {
-            const bool empty = M == -INFINITY && S == 0.f;
-            const float ls = empty ? 0.f : logf(S);
-            const float H = empty ? 0.f : ls - Tw / S;
-            const int64_t y = tokens[r];
-            float lp = 0.f;
-            if (y != ignore_index)
-                lp = (y < 0 || y >= V) ? NAN : empty ? -INFINITY : (gf_to_f<D>(logits[r * row_stride + y]) - M) * c - ls;
-            logp[r] = lp;
-            if (entropy) entropy[r] = H;
-            if (stats) stats[r * 3] = M, stats[r * 3 + 1] = ls, stats[r * 3 + 2] = H;
+            answer_row<D>(ans, r, logits + r * row_stride, V, c, M, S, Tw, ls);
             s_row[0] = M;
             s_row[1] = ls;
         }
     }
     if (top == 0) return;
     if (tid < top) s_best[tid] = 0ull;
-    __syncthreads();
     const int64_t total = (int64_t)tiles * top;
-    for (int64_t k0 = 0; k0 < total; k0 += 2048) {              // the tiles' best keys in pieces, with the best ones so far
-        const int n0 = (int)(total - k0 < 2048 ? total - k0 : 2048), n = n0 + top;
-        for (int i = tid; i < n; i += kThr) s_key[i] = i < top ? s_best[i] : in.keys[r * total + k0 + i - top];
+    const u64* keys = in.keys + r * total;
+    for (int64_t k0 = 0; k0 < total; k0 += kPer * kThr) {       // the tiles' best keys in pieces, with the best ones so far; chosen as in a tile
+        u64 key[kPer + 1], best = 0ull;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            const int64_t k = k0 + i * kThr + tid;
+            key[i] = k < total ? keys[k] : 0ull;
+        }
+        if (tid == 0) s_n = 0;
         __syncthreads();
+        key[kPer] = tid < top ? s_best[tid] : 0ull;
+#pragma unroll
+        for (int i = 0; i <= kPer; ++i) best = key[i] > best ? key[i] : best;
+        const unsigned o = (unsigned)(best >> 32);
+        const unsigned a = kth_of_wave(o, (top + 3) / 4), b = kth_of_wave(o, top);
+        if (lane == 0) s_thr[wave] = a, s_thr[4 + wave] = b;
+        __syncthreads();
+        unsigned ua = s_thr[0], ub = s_thr[4];
+#pragma unroll
+        for (int w = 1; w < 4; ++w) ua = min(ua, s_thr[w]), ub = max(ub, s_thr[4 + w]);
+        const unsigned u = max(ua, ub);
         if (tid < top) s_best[tid] = 0ull;
+#pragma unroll
+        for (int i = 0; i <= kPer; ++i)
+            if (key[i] != 0ull && (unsigned)(key[i] >> 32) >= u) s_cand[atomicAdd(&s_n, 1)] = key[i];
         __syncthreads();
+        const int n = s_n;
         for (int i = tid; i < n; i += kThr) {
-            const u64 key = s_key[i];
-            if (key == 0ull) continue;
-            int rank = 0;
-            for (int q = 0; q < n; ++q) rank += s_key[q] > key;
-            if (rank < top) s_best[rank] = key;
+            const u64 k = s_cand[i];
+            const int rank = rank_of(s_cand, n, k);
+            if (rank < top) s_best[rank] = k;
         }
         __syncthreads();
     }
-    if (tid < top) {
-        const u64 key = s_best[tid];
-        const int64_t j = (unsigned)~(unsigned)key;
-        const unsigned o = (unsigned)(key >> 32);
-        const float x = o == 0xfffffffeu ? NAN : unord32(o), M = s_row[0];
-        top_tokens[r * top + tid] = j;
-        top_logp[r * top + tid] = (M == -INFINITY && s_row[1] == 0.f) ? -INFINITY : (x - M) * c - s_row[1];
-    }
+    if (tid < top) answer_top(ans, r * top + tid, s_best[tid], c, s_row[0], s_row[1]);
 }
 
 // ---- gradients: dlogits = f(x) for every output, then the named ones over it ------------------------------------------------
@@ -362,7 +471,7 @@ __global__ __launch_bounds__(kThr) void token_bwd_kernel(const D* __restrict__ l
     D* drow = dlogits + r * V;
     const bool none = A == 0.f && gH == 0.f;
     auto base = [&](float x) {
-        const float lp = (x - m) * c - ls, p = exp2f(lp * kLog2e);
+        const float lp = (x - m) * c - ls, p = exp2_fast(lp * kLog2e);
         return (none || p == 0.f) ? 0.f : -c * p * fmaf(gH, lp + H, A);
     };
     for_tile<D>(row, drow, g0, groups, base);
@@ -386,7 +495,7 @@ __global__ __launch_bounds__(kThr) void distill_finish_kernel(const D* __restric
     const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (r >= R) return;
     float M, S, Tw;
-    join_tiles(in, r, tiles, c, lane, M, S, Tw);
+    join_tiles(in, r, tiles, c, lane, false, M, S, Tw);
     int64_t j = -1;
     double v = -INFINITY, x = 0.0;
     if (lane < K) {
@@ -417,11 +526,12 @@ __global__ __launch_bounds__(kThr) void distill_finish_kernel(const D* __restric
     some = tail ? __ballot(on) != 0ull : some;
     double mine = 0.0;                                          // mass of my output
     bool first = true;
+    const int ji = (int)j;                                      // (V < 2^31)
     for (int k = 0; k < K; ++k) {
-        const int64_t jk = __shfl(j, k);
-        const double pk = __shfl(p, k);
-        if (jk == j) mine += pk;
-        if (jk == j && k < lane) first = false;
+        const int jk = __builtin_amdgcn_readlane(ji, k);
+        const double pk = lane_value(p, k);
+        if (jk == ji) mine += pk;
+        if (jk == ji && k < lane) first = false;
     }
     if (!tail) {
         const double ls = log((double)S);
@@ -490,7 +600,7 @@ __global__ __launch_bounds__(kThr) void distill_bwd_kernel(const D* __restrict__
     D* drow = dlogits + r * V;
     const bool none = g == 0.f || w == 0.f || (m == -INFINITY && ls == -INFINITY);   // (the second: every output named or ruled out)
     for_tile<D>(row, drow, g0, groups, [&](float x) {
-        const float p = exp2f(((x - m) * c - ls) * kLog2e);
+        const float p = exp2_fast(((x - m) * c - ls) * kLog2e);
         return none ? 0.f : w * p;
     });
     __syncthreads();                                            // (the workgroup's own stores are done: the named outputs follow them)
@@ -501,16 +611,14 @@ __global__ __launch_bounds__(kThr) void distill_bwd_kernel(const D* __restrict__
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------------
-// groups (16-byte vectors) per thread of a tile: as large as the registers hold (8) once that gives the chip enough workgroups
+// groups (16-byte vectors) per thread of a tile: up to kMaxNV once that gives the chip enough workgroups
 template <typename D> int pick_nv(int64_t R, int64_t V) {
     const int64_t groups = row_groups<D>(V);
-    for (int nv = 8; nv > 1; nv >>= 1) {
+    for (int nv = kMaxNV; nv > 1; nv >>= 1) {
         const int64_t tiles = (groups + (int64_t)nv * kThr - 1) / ((int64_t)nv * kThr);
         if (R * tiles >= 2048 && groups > (int64_t)(nv / 2) * kThr) return nv;
     }
-    int nv = 1;                                                 // few rows: small tiles; a single one where it suffices
-    while (nv < 8 && (groups + (int64_t)nv * kThr - 1) / ((int64_t)nv * kThr) * R > 4096) nv <<= 1;
-    return nv;
+    return groups > 64 * kThr ? 2 : 1;                          // few rows: small tiles, yet not so many that joining them counts
 }
 template <typename D> int64_t tiles_of(int64_t V, int nv) { return (row_groups<D>(V) + (int64_t)nv * kThr - 1) / ((int64_t)nv * kThr); }
 
@@ -528,18 +636,14 @@ Parts make_parts(void* ws, int64_t R, int64_t tiles, int top) {
     return p;
 }
 
-template <typename D, bool TOP, bool MASK>
-int run_tiles(const void* logits, int64_t row_stride, int64_t R, int V, float c, int top, const int64_t* indices, int K, const Parts& parts,
-              hipStream_t st) {
-    const int nv = pick_nv<D>(R, V);
-    const int tiles = (int)tiles_of<D>(V, nv);
+template <typename D, bool TOP, bool ENT, bool MASK, bool ONE>
+int run_tiles(const void* logits, int64_t row_stride, int64_t R, int V, int nv, int tiles, float c, int top, const int64_t* indices, int K,
+              const Parts& parts, const TokenOut& ans, hipStream_t st) {
     const dim3 grid((unsigned)(R * tiles));
     const D* x = static_cast<const D*>(logits);
-    const float c2 = c * kLog2e;
-    if (nv == 8) tile_kernel<D, 8, TOP, MASK><<<grid, kThr, 0, st>>>(x, row_stride, V, tiles, c2, top, indices, K, parts);
-    else if (nv == 4) tile_kernel<D, 4, TOP, MASK><<<grid, kThr, 0, st>>>(x, row_stride, V, tiles, c2, top, indices, K, parts);
-    else if (nv == 2) tile_kernel<D, 2, TOP, MASK><<<grid, kThr, 0, st>>>(x, row_stride, V, tiles, c2, top, indices, K, parts);
-    else tile_kernel<D, 1, TOP, MASK><<<grid, kThr, 0, st>>>(x, row_stride, V, tiles, c2, top, indices, K, parts);
+    if (nv == 4) tile_kernel<D, 4, TOP, ENT, MASK, ONE><<<grid, kThr, 0, st>>>(x, row_stride, V, tiles, c, top, indices, K, parts, ans);
+    else if (nv == 2) tile_kernel<D, 2, TOP, ENT, MASK, ONE><<<grid, kThr, 0, st>>>(x, row_stride, V, tiles, c, top, indices, K, parts, ans);
+    else tile_kernel<D, 1, TOP, ENT, MASK, ONE><<<grid, kThr, 0, st>>>(x, row_stride, V, tiles, c, top, indices, K, parts, ans);
     GF_LAUNCH_CHECK("tile_kernel");
     return GF_OK;
 }
@@ -566,13 +670,16 @@ template <typename D> void bwd_tiles(int64_t R, int64_t V, int& tiles, int& grou
 template <typename D>
 int token_forward_t(const void* logits, int64_t row_stride, const int64_t* tokens, float c, int64_t ignore, float* logp, float* entropy, float* top_logp,
                     int64_t* top_tokens, int top, float* stats, void* ws, int64_t R, int V, hipStream_t st) {
-    const int tiles = (int)tiles_of<D>(V, pick_nv<D>(R, V));
+    const int nv = pick_nv<D>(R, V), tiles = (int)tiles_of<D>(V, nv);
     const Parts p = make_parts(ws, R, tiles, top);
-    const int rc = top ? run_tiles<D, true, false>(logits, row_stride, R, V, c, top, nullptr, 0, p, st)
-                       : run_tiles<D, false, false>(logits, row_stride, R, V, c, 0, nullptr, 0, p, st);
+    const TokenOut a{tokens, ignore, logp, entropy, top_logp, top_tokens, stats};
+    if (tiles == 1)
+        return top ? run_tiles<D, true, true, false, true>(logits, row_stride, R, V, nv, 1, c, top, nullptr, 0, p, a, st)
+                   : run_tiles<D, false, true, false, true>(logits, row_stride, R, V, nv, 1, c, 0, nullptr, 0, p, a, st);
+    const int rc = top ? run_tiles<D, true, true, false, false>(logits, row_stride, R, V, nv, tiles, c, top, nullptr, 0, p, a, st)
+                       : run_tiles<D, false, true, false, false>(logits, row_stride, R, V, nv, tiles, c, 0, nullptr, 0, p, a, st);
     if (rc != GF_OK) return rc;
-    token_finish_kernel<D><<<dim3((unsigned)R), dim3(top ? kThr : 64), 0, st>>>(static_cast<const D*>(logits), row_stride, tokens, c, ignore, p, tiles, V,
-                                                                                top, logp, entropy, top_logp, top_tokens, stats);
+    token_finish_kernel<D><<<dim3((unsigned)R), dim3(top ? kThr : 64), 0, st>>>(static_cast<const D*>(logits), row_stride, c, p, tiles, V, top, a);
     GF_LAUNCH_CHECK("token_finish_kernel");
     return GF_OK;
 }
@@ -591,10 +698,11 @@ int token_backward_t(const void* logits, int64_t row_stride, const int64_t* toke
 template <typename D>
 int distill_forward_t(const void* logits, int64_t row_stride, const int64_t* indices, const float* values, float c, int tail, float* loss, float* stats,
                       float* probs, void* ws, int64_t R, int V, int K, hipStream_t st) {
-    const int tiles = (int)tiles_of<D>(V, pick_nv<D>(R, V));
+    const int nv = pick_nv<D>(R, V), tiles = (int)tiles_of<D>(V, nv);
     const Parts p = make_parts(ws, R, tiles, 0);
-    const int rc = tail ? run_tiles<D, false, true>(logits, row_stride, R, V, c, 0, indices, K, p, st)
-                        : run_tiles<D, false, false>(logits, row_stride, R, V, c, 0, nullptr, 0, p, st);
+    const TokenOut none{};
+    const int rc = tail ? run_tiles<D, false, false, true, false>(logits, row_stride, R, V, nv, tiles, c, 0, indices, K, p, none, st)
+                        : run_tiles<D, false, false, false, false>(logits, row_stride, R, V, nv, tiles, c, 0, nullptr, 0, p, none, st);
     if (rc != GF_OK) return rc;
     distill_finish_kernel<D><<<dim3((unsigned)((R + 3) / 4)), kThr, 0, st>>>(static_cast<const D*>(logits), row_stride, indices, values, c, tail, p, tiles,
                                                                              R, V, K, loss, stats, probs);

@@ -60,6 +60,7 @@ def recurrence_bounds(u, qc, qh, z0, lengths, dz, dzT, dtype):
 
 
 # ---- tokens and distillation: definitions in float64, row by row, with bounds -------------------------------------------------------
+FLUSH = 2.0 ** -126  # the exponential gives zero for results below 2^-126: a probability is off by less than that, its gradient by that times its weight
 NSUM = 320           # roundings of a term of a row's sums, at most: 64 in a thread, 10 in a workgroup, the tiles' joins, the exponential's own
 
 
@@ -122,7 +123,7 @@ def tokens(x, tok, top, T, ignore, dlogp, dent, dtop, half):
         d = c * (w - p * w.sum() - gH * p * (lpz + H))
         rel = dlp + 8 * U
         err = c * (p * (rel * (abs(w.sum()) + abs(gH) * np.abs(lpz + H)) + (top + 4) * U * wa.sum() + abs(gH) * (dlp + dH + 4 * U * (np.abs(lpz) + H)))
-                   + 6 * U * wa)
+                   + 6 * U * wa + FLUSH * (abs(w.sum()) + abs(gH) * (np.abs(lpz) + H)))
         out["dlogits"][r], tol["dlogits"][r] = d, 1.05 * err + half[0] * 1.01 * np.abs(d) + half[1]
     return out, tol
 
@@ -160,7 +161,7 @@ def distill(x, idx, val, T, tail, dloss, half):
         g = dloss[r] * c
         if not tail:
             d = g * (q - mass)
-            err = abs(g) * (q * (dlq + 8 * U) + masserr) + 4 * U * np.abs(d)
+            err = abs(g) * (q * (dlq + 8 * U) + masserr + FLUSH) + 4 * U * np.abs(d)
             el = (p * dlq[i]).sum() + (p * dp * (np.abs(lp - np.where(p > 0, lq[i], 0.0)) + 1)).sum()
         else:
             W = 1.0 if pr > 0 else p.sum()
@@ -174,7 +175,7 @@ def distill(x, idx, val, T, tail, dloss, half):
             d = g * np.where(named, W * q - mass, rest * coef)
             ey = 4 * U * np.abs(np.where(np.isfinite(y), y, 0.0))
             share = qr * (1 - qr) * (esr + ey[i].max() + 4 * U * abs(ls))                      # of q_r
-            err = abs(g) * np.where(named, q * (ey + esr + 8 * U), rest * (abs(coef) * (4 * U * np.abs(yr) + esr + 12 * U) + share)) + 4 * U * np.abs(d)
+            err = abs(g) * np.where(named, q * (ey + esr + 8 * U), rest * (abs(coef) * (4 * U * np.abs(yr) + esr + 12 * U) + share) + FLUSH * abs(coef)) + 4 * U * np.abs(d)
             el = abs(coef) * esr + (np.abs(W * q[i] - mass[i]) * ey[i]).sum() + 1e-12
         out["loss"][r], tol["loss"][r] = loss, (1.05 * el + 3 * U * abs(loss) if np.isfinite(loss) else 0.0)
         out["dlogits"][r], tol["dlogits"][r] = d, 1.05 * err + half[0] * 1.01 * np.abs(d) + half[1]
