@@ -10,6 +10,8 @@ Layout mirrors the reference package so that call sites read the same:
                                                                                                      GraphRecurrentNN)
     alegnn.modules.{model,training,evaluation}  ->  alegnn_amd.modules.{model,training,evaluation}  (Trainer with batch DP;
                                                     losses: any torch loss or the reference's own alegnn.modules.loss wrapper)
+Beyond the reference: linear_recurrence (a recurrent layer parallel in time: utils.graphML.LinearHiddenState), token_log_probs (answers with
+probabilities and alternatives: modules.evaluation.predictTop) and distill_top (learning from those: Trainer's teacherTop).
 `install(reference_gml)` rebinds the reference's own symbols.
 """
 from .functional import EVGF_edges, LSIGF

@@ -8,6 +8,7 @@ one filter per step; the gates are GatedGRNN's q_hat / q_check (time, node) and,
 from __future__ import annotations
 
 import contextlib
+import functools
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -51,36 +52,38 @@ def _dense(t):
 
 
 def _gate_kind(q, shape, name):
-    assert q.dim() == 4 and q.shape[1] == shape[1], f"{name}: shape {tuple(q.shape)} for an input {tuple(shape)} (want [B|1, T, H|1, N|1])"
-    kind = 0
-    for axis, bit in ((0, _lib.GF_GATE_B), (2, _lib.GF_GATE_H), (3, _lib.GF_GATE_N)):
-        assert q.shape[axis] in (1, shape[axis]), f"{name}: shape {tuple(q.shape)} for an input {tuple(shape)} (want [B|1, T, H|1, N|1])"
-        if q.shape[axis] == shape[axis]:
-            kind |= bit
-    return kind
+    """Which axes a gate of an input [B, T, H, N] has (GF_GATE_*)."""
+    have = tuple(q.shape)
+    B, T, H, N = shape
+    if not (len(have) == 4 and have[1] == T and have[0] in (1, B) and have[2] in (1, H) and have[3] in (1, N)):
+        raise AssertionError(f"{name}: shape {have} for an input {tuple(shape)} (want [B|1, T, H|1, N|1])")
+    return (_lib.GF_GATE_B if have[0] == B else 0) | (_lib.GF_GATE_H if have[2] == H else 0) | (_lib.GF_GATE_N if have[3] == N else 0)
 
 
-def _forward(u, qc, qh, z0, lengths, keep):
+@functools.lru_cache(maxsize=256)
+def _sizes(B, T, H, N, kc, hat, kh):
+    """(checkpoint floats, forward workspace bytes, backward workspace bytes) of a shape."""
+    L = _lib.lib()
+    return (L.gf_recurrence_checkpoint_floats(B, T, H, N, kc, hat, kh), L.gf_recurrence_workspace_bytes(B, T, H, N, kc, hat, kh, 0),
+            L.gf_recurrence_workspace_bytes(B, T, H, N, kc, hat, kh, 1))
+
+
+def _forward(u, qc, qh, z0, lengths, kinds, keep):
     L = _lib.lib()
     B, T, H, N = u.shape
     dev = u.device
-    kc = _gate_kind(qc, u.shape, "q_check")
-    kh = 0 if qh is None else _gate_kind(qh, u.shape, "q_hat")
-    hat = 0 if qh is None else 1
+    kc, kh, hat = kinds
     with _on(dev):
         z = torch.empty((B, T, H, N), dtype=u.dtype, device=dev)
         zT = torch.empty((B, H, N), dtype=torch.float32, device=dev)
-        if u.numel() == 0 and B * H * N == 0:
-            return z, zT, None, (kc, kh, hat)
-        ckpt = None
-        if keep:
-            ckpt = torch.empty(L.gf_recurrence_checkpoint_floats(B, T, H, N, kc, hat, kh), dtype=torch.float32, device=dev)
-        nb = L.gf_recurrence_workspace_bytes(B, T, H, N, kc, hat, kh, 0)
-        ws = torch.empty(nb // 4, dtype=torch.float32, device=dev) if nb else None
+        if B * H * N == 0:
+            return z, zT, None
+        nck, nb, _ = _sizes(B, T, H, N, kc, hat, kh)
+        ckpt = torch.empty(nck, dtype=torch.float32, device=dev) if keep else None
+        ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
         _lib.check(L.gf_recurrence_forward(u.data_ptr(), qc.data_ptr(), kc, _ptr(qh), kh, _ptr(z0), _ptr(lengths), z.data_ptr(), zT.data_ptr(),
-                                           _ptr(ckpt), _ptr(ws), nb, _DTYPES[u.dtype], B, T, H, N, _stream(dev)),
-                   "gf_recurrence_forward")
-    return z, zT, ckpt, (kc, kh, hat)
+                                           _ptr(ckpt), _ptr(ws), nb, _DTYPES[u.dtype], B, T, H, N, _stream(dev)), "gf_recurrence_forward")
+    return z, zT, ckpt
 
 
 def _once(f, ctx, *grads):
@@ -96,7 +99,7 @@ def _recurrence_backward(ctx, dz, dzT):
     dev = u.device
     need_u, need_c, need_h, need_0 = ctx.needs_input_grad[:4]
     if dz is None and dzT is None:
-        return None, None, None, None, None
+        return None, None, None, None, None, None
     dz, dzT = _dense(dz), _dense(dzT)
     with _on(dev):
         du = torch.empty_like(u) if need_u else None
@@ -104,22 +107,23 @@ def _recurrence_backward(ctx, dz, dzT):
         dqh = torch.empty_like(qh) if need_h else None
         dz0 = torch.empty((B, H, N), dtype=torch.float32, device=dev) if need_0 else None
         if B * H * N == 0:
-            return du, None if dqc is None else dqc.zero_(), None if dqh is None else dqh.zero_(), dz0, None
-        nb = L.gf_recurrence_workspace_bytes(B, T, H, N, kc, hat, kh, 1)
-        ws = torch.empty(nb // 4, dtype=torch.float32, device=dev) if nb else None
+            return du, None if dqc is None else dqc.zero_(), None if dqh is None else dqh.zero_(), dz0, None, None
+        nb = _sizes(B, T, H, N, kc, hat, kh)[2]
+        ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
         _lib.check(L.gf_recurrence_backward(u.data_ptr(), qc.data_ptr(), kc, _ptr(qh), kh, _ptr(lengths), _ptr(ckpt), _ptr(dz), _ptr(dzT),
                                             _ptr(du), _ptr(dqc), _ptr(dqh), _ptr(dz0), _ptr(ws), nb, _DTYPES[u.dtype], B, T, H, N,
                                             _stream(dev)), "gf_recurrence_backward")
-    return du, dqc, dqh, dz0, None
+    return du, dqc, dqh, dz0, None, None
 
 
 class _LinearRecurrenceFunction(torch.autograd.Function):
     """gf_recurrence_forward / gf_recurrence_backward (include/gfhip.h)."""
 
     @staticmethod
-    def forward(ctx, u, qc, qh, z0, lengths):
+    def forward(ctx, u, qc, qh, z0, lengths, kinds):
         u, qc, qh, z0 = _dense(u), _dense(qc), _dense(qh), _dense(z0)
-        z, zT, ckpt, ctx.kinds = _forward(u, qc, qh, z0, lengths, ctx.needs_input_grad[1])
+        z, zT, ckpt = _forward(u, qc, qh, z0, lengths, kinds, ctx.needs_input_grad[1])
+        ctx.kinds = kinds
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(u, qc, qh, lengths, ckpt)
         return z, zT
@@ -141,11 +145,13 @@ def linear_recurrence(u, q_check, q_hat=None, z0=None, lengths=None):
     who = "linear_recurrence"
     assert u.dim() == 4, f"{who}: u has shape {tuple(u.shape)}, want [B, T, H, N]"
     _require_cuda(who, "u", u, _FLOATS)
-    for name, q in (("q_check", q_check), ("q_hat", q_hat)):
+    kinds = [0, 0, 0 if q_hat is None else 1]
+    for i, name, q in ((0, "q_check", q_check), (1, "q_hat", q_hat)):
         if q is not None:
-            _gate_kind(q, u.shape, name)
+            kinds[i] = _gate_kind(q, u.shape, name)
             _require_cuda(who, name, q, (u.dtype,))
             assert q.device == u.device, f"{who}: {name} is on {q.device}, u on {u.device}"
+    kinds = tuple(kinds)
     if z0 is not None:
         assert tuple(z0.shape) == (u.shape[0], u.shape[2], u.shape[3]), f"{who}: z0 has shape {tuple(z0.shape)} for u {tuple(u.shape)}"
         _require_cuda(who, "z0", z0, _F32)
@@ -156,6 +162,5 @@ def linear_recurrence(u, q_check, q_hat=None, z0=None, lengths=None):
         assert lengths.device == u.device, f"{who}: lengths is on {lengths.device}, u on {u.device}"
         lengths = lengths.contiguous()
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (u, q_check, q_hat, z0)):
-        return _LinearRecurrenceFunction.apply(u, q_check, q_hat, z0, lengths)
-    z, zT, _, _ = _forward(_dense(u), _dense(q_check), _dense(q_hat), _dense(z0), lengths, False)
-    return z, zT
+        return _LinearRecurrenceFunction.apply(u, q_check, q_hat, z0, lengths, kinds)
+    return _forward(_dense(u), _dense(q_check), _dense(q_hat), _dense(z0), lengths, kinds, False)[:2]

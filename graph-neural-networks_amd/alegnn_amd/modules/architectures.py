@@ -466,10 +466,11 @@ class GraphRecurrentNN(nn.Module):
     (``hiddenState``, ``outputState``, ``Readout``) and state_dict keys.  x: B x T x F x N -> B x T x dimReadout[-1] x N.
 
     The reference draws the initial state inside splitForward (``torch.randn`` on x's device, :4556); ``z0`` can be passed
-    instead (superset) so that a run is reproducible across devices."""
+    instead (superset) so that a run is reproducible across devices.  ``hiddenLayer`` (superset) is the recurrent layer's class,
+    called as HiddenState is: gml.LinearHiddenState runs all time steps in parallel."""
 
     def __init__(self, dimInputSignals, dimOutputSignals, dimHiddenSignals, nFilterTaps, bias, nonlinearityHidden,
-                 nonlinearityOutput, nonlinearityReadout, dimReadout, GSO):
+                 nonlinearityOutput, nonlinearityReadout, dimReadout, GSO, hiddenLayer=gml.HiddenState):
         super().__init__()
         assert len(nFilterTaps) == 2                                # :4463
         self.F = dimInputSignals
@@ -482,7 +483,7 @@ class GraphRecurrentNN(nn.Module):
         self.nonlinearityReadout = nonlinearityReadout
         self.dimReadout = dimReadout
         self._install(GSO)
-        self.hiddenState = gml.HiddenState(self.F, self.H, self.K[0], nonlinearity=self.sigma, E=self.E, bias=self.bias)
+        self.hiddenState = hiddenLayer(self.F, self.H, self.K[0], nonlinearity=self.sigma, E=self.E, bias=self.bias)
         self.outputState = gml.GraphFilter(self.H, self.G, self.K[1], E=self.E, bias=self.bias)
         self.hiddenState.addGSO(self._gso)
         self.outputState.addGSO(self._gso)

@@ -1,4 +1,4 @@
-"""evaluate / evaluateSingleNode -- the reference's alegnn/modules/evaluation.py:18-168.
+"""evaluate / evaluateSingleNode -- the reference's alegnn/modules/evaluation.py:18-168; predictTop: a classifier's answers in full.
 
 Test-set cost of the 'Best' and the 'Last' checkpoint; returns {'costBest', 'costLast'} and (doSaveVars) pickles it to
 <saveDir>/evalVars/<name>evalVars.pkl.  Under torch.distributed every rank evaluates its identical replica; rank 0 writes.
@@ -10,6 +10,8 @@ import pickle
 
 import torch
 import torch.distributed as dist
+
+from ..functional_out import token_log_probs
 
 
 def _run(model, data, forward, kwargs):
@@ -40,3 +42,20 @@ def evaluateSingleNode(model, data, **kwargs):
     assert 'getLabelID' in dir(data)
     targetIDs = data.getLabelID('test')
     return _run(model, data, lambda x: model.archit.singleNodeForward(x, targetIDs), kwargs)
+
+
+def predictTop(model, data, samplesType='test', top=5, temperature=1.0, batchSize=None):
+    """What the model's architecture, as it stands, answers on a split of a classification data set (outputs B x classes, labels B): a dict of
+    'logProb' [B] (of the true class), 'entropy' [B], and the `top` best classes per sample 'topLogProb' / 'topClasses' [B, top], under
+    softmax(output / temperature).  (topClasses, topLogProb) of the training split is what Trainer takes as teacherTop."""
+    x, y = data.getSamples(samplesType)
+    n = x.shape[0]
+    step = n if batchSize is None else int(batchSize)
+    parts = []
+    with torch.no_grad():
+        for b in range(0, n, step):
+            out = model.archit(x[b:b + step].to(model.device))
+            labels = y[b:b + step].to(model.device).to(torch.int64).reshape(out.shape[0])
+            parts.append(token_log_probs(out, labels, top=min(int(top), out.shape[1]), temperature=temperature))
+    names = ('logProb', 'entropy', 'topLogProb', 'topClasses')
+    return {k: None if parts[0][i] is None else torch.cat([p[i] for p in parts]) for i, k in enumerate(names)}

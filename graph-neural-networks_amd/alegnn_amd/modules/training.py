@@ -16,6 +16,11 @@ identical replica.  Per step
 Validation is computed by every rank on the full validation set (identical replicas -> identical decisions, no exchange);
 checkpoints are written by rank 0 (model.py).
 
+``teacherTop=(classes, logProbs)`` (superset option): two [nTrain, K] tensors, the K best classes of a teacher for every training sample with
+their log probabilities (evaluation.predictTop of the training split, K <= 64, an index outside the classes = padding).  A step then minimises
+(1 - distillWeight) * loss + distillWeight * mean distill_top(output, classes, logProbs) with what the K classes leave as one further outcome
+(distillWeight 0.5, distillTemperature 1.0: the temperature the log probabilities were taken at).  Validation keeps the plain loss.
+
 ``hipGraph=True`` (superset option, GPU only): zero-grad + forward + loss + backward of a training step are captured once per
 batch size as a HIP graph and replayed; the samples are copied into the graph's static input buffers, the (all-reduce and)
 optimizer step stay eager.  The reference's own configurations (N = 100 nodes, batch 20-100) are launch-bound -- about forty
@@ -33,6 +38,7 @@ import numpy as np
 import torch
 import torch.distributed as dist
 
+from ..functional_out import distill_top
 from ..parallel import GradBucket, broadcast, broadcast_parameters
 
 
@@ -94,6 +100,16 @@ class Trainer:
             self.trainingOptions['learningRateDecayRate'] = kwargs['learningRateDecayRate']
             self.trainingOptions['learningRateDecayPeriod'] = kwargs['learningRateDecayPeriod']
 
+        self.teacher = None
+        if kwargs.get('teacherTop') is not None:
+            classes, logProbs = kwargs['teacherTop']
+            if classes.shape != logProbs.shape or classes.dim() != 2 or classes.shape[0] != nTrain:
+                raise ValueError(f"teacherTop: two [nTrain, K] tensors wanted, got {tuple(classes.shape)} and {tuple(logProbs.shape)} for nTrain = {nTrain}")
+            self.teacher = (classes.detach().to(torch.int64), logProbs.detach().float())
+            self.distillWeight = float(kwargs.get('distillWeight', 0.5))
+            self.distillTemperature = float(kwargs.get('distillTemperature', 1.0))
+            if not 0.0 <= self.distillWeight <= 1.0:
+                raise ValueError(f"distillWeight: {self.distillWeight} is not in [0, 1]")
         self.useGraph = bool(kwargs.get('hipGraph', False))
         self._graphs = {}                                           # batch size -> captured step
         self.bucket = None
@@ -111,6 +127,21 @@ class Trainer:
 
     def _forward(self, x, samplesType, indices):
         return self.model.archit(x)
+
+    def _teacher_rows(self, indices):
+        """The teacher's entries of these training samples on the model's device (None without a teacher)."""
+        if self.teacher is None:
+            return None
+        rows = torch.as_tensor(indices, dtype=torch.int64)
+        dev = torch.device(self.model.device)
+        return tuple(t[rows.to(t.device)].to(dev) for t in self.teacher)
+
+    def _loss(self, yHat, y, teacher):
+        lossValue = self.model.loss(yHat, y)
+        if teacher is None:
+            return lossValue
+        w = self.distillWeight
+        return (1.0 - w) * lossValue + w * distill_top(yHat, *teacher, temperature=self.distillTemperature, tail=True).mean()
 
     # ---- the step as a HIP graph (hipGraph=True) ---------------------------------------------------------------------
     def _graph_step(self, xTrain, yTrain, samplesType, indices, weight):
@@ -134,6 +165,7 @@ class Trainer:
             sy = torch.empty(yTrain.shape, dtype=yTrain.dtype, device=dev)
             sx.copy_(xTrain)
             sy.copy_(yTrain)
+            st = self._teacher_rows(indices)                        # static too: refilled before every replay
             params = [p for p in self.model.archit.parameters() if p.requires_grad]
 
             def body():
@@ -143,7 +175,7 @@ class Trainer:
                 else:
                     self.bucket.zero_()
                 yHat = self._forward(sx, samplesType, indices)
-                lossValue = self.model.loss(yHat, sy)
+                lossValue = self._loss(yHat, sy, st)
                 (lossValue * weight if self.world > 1 else lossValue).backward()
                 return lossValue, yHat
 
@@ -156,10 +188,13 @@ class Trainer:
             graph = torch.cuda.CUDAGraph()
             with torch.cuda.graph(graph):
                 out = body()
-            g = self._graphs[key] = dict(graph=graph, x=sx, y=sy, out=out, weight=weight, gsos=gsos,
+            g = self._graphs[key] = dict(graph=graph, x=sx, y=sy, teacher=st, out=out, weight=weight, gsos=gsos,
                                          grads=[p.grad for p in params], params=params)
         g["x"].copy_(xTrain, non_blocking=True)
         g["y"].copy_(yTrain, non_blocking=True)
+        if g["teacher"] is not None:
+            for static, rows in zip(g["teacher"], self._teacher_rows(indices)):
+                static.copy_(rows, non_blocking=True)
         g["graph"].replay()
         if self.bucket is None:
             for p, gr in zip(g["params"], g["grads"]):
@@ -194,7 +229,7 @@ class Trainer:
             xTrain = xTrain.to(self.model.device)
             yTrain = yTrain.to(self.model.device)
             yHatTrain = self._forward(xTrain, 'train', mine)        # :244
-            lossValueTrain = self.model.loss(yHatTrain, yTrain)     # :247
+            lossValueTrain = self._loss(yHatTrain, yTrain, self._teacher_rows(mine))     # :247
             weight = len(mine) * self.world / len(thisBatchIndices)
             (lossValueTrain * weight if self.world > 1 else lossValueTrain).backward()      # :250
             lossValue = lossValueTrain.item() * weight

@@ -11,6 +11,7 @@ Drop-in for the symbols SelectionGNN binds from alegnn/utils/graphML.py:
     NVGF           (graphML.py:293-387)    -> alegnn_amd.functional.NVGF  (HIP: LSIGF's tap stack, per-node bank)
     NodeVariantGF  (graphML.py:2317-2509)  the module around it (NodeVariantGNN's layer)
     LSIGF_DB / GRNN_DB / GraphFilter_DB / HiddenState_DB (graphML.py:977-1290, 3278-3538)  per-sample, delayed GSOs (gf_db.hip)
+    LinearGRNN / LinearHiddenState  (superset) recurrent layer that is linear in its state: all time steps in parallel (gf_recur.hip)
     EdgeGatedHiddenState (graphML.py:4033-4208) and the edge-gated branches of GatedGRNN (:1394-1419, :1434-1456)
     NoPool         (graphML.py:1850-1888)  identity pooling
     MaxPoolLocal   (graphML.py:1890-2028)  alpha-hop neighbourhood max, keep the first nOutputNodes nodes
@@ -28,12 +29,13 @@ import torch.nn as nn
 
 from ..functional import EVGF_edges, LSIGF, NVGF, expand_node_taps, max_pool_local
 from ..functional_db import GRNN_DB, LSIGF_DB, filter_per_sample
+from ..functional_seq import linear_recurrence
 from ..gso import EdgePattern, SparseGSO
 from . import graphTools
 
 __all__ = ["LSIGF", "GraphFilter", "EdgeVariantGF", "NoPool", "MaxPoolLocal", "FusedReLU", "GatedGRNN", "HiddenState", "TimeGatedHiddenState",
            "NodeGatedHiddenState", "EdgeGatedHiddenState", "jARMA", "NVGF", "NodeVariantGF", "LSIGF_DB", "GRNN_DB", "GraphFilter_DB",
-           "HiddenState_DB", "learnAttentionGSO", "GraphAttentional"]
+           "HiddenState_DB", "learnAttentionGSO", "GraphAttentional", "LinearGRNN", "LinearHiddenState"]
 
 
 class FusedReLU(nn.Identity):
@@ -482,6 +484,88 @@ class HiddenState(nn.Module):
     def extra_repr(self):
         reprString = "in_features=%d, hidden_features=%d, " % (self.F, self.H) + "filter_taps=%d, " % (self.K) + \
                      "edge_features=%d, " % (self.E) + "bias=%s, " % (self.bias) + "nonlinearity=%s" % (self.sigma)
+        reprString += "GSO stored" if self.S is not None else "no GSO stored"
+        return reprString
+
+
+def LinearGRNN(a, S, x, z0, sigma, q_hat, q_check, xBias=None, lengths=None):
+    """Hidden states z_t = q_check_t * z_{t-1} + q_hat_t * sigma(A(S) x_t), t = 1..T: GatedGRNN (graphML.py:1292-1527) with a state that is carried
+    by its gate alone, so that all T steps run in parallel (two launches instead of a filter per step).
+
+    a [H,E,K,F] input-to-hidden taps, S the GSO, x [B,T,F,N], z0 [B,H,N] or None, gates [B|1, T, H|1, N|1] (q_hat None = 1), xBias [H,1];
+    lengths [B] int32 = steps of each sequence that count (None = all).  Returns (z [B,T,H,N], z_T [B,H,N])."""
+    H, E, K, F = a.shape
+    gso = SparseGSO.from_any(S)
+    B, T, N = x.shape[0], x.shape[1], gso.N
+    assert x.shape[2] == F and x.shape[3] == N
+    Ax = LSIGF(a, gso, x.reshape(B * T, F, N), xBias).reshape(B, T, H, N)
+    return linear_recurrence(Ax if sigma is None else sigma(Ax), q_check, q_hat, z0, lengths)
+
+
+class LinearHiddenState(nn.Module):
+    """LinearHiddenState(signal_features, hidden_features, filter_taps, nonlinearity=torch.tanh, edge_features=1, bias=True, gate='element')
+    -- a recurrent layer beside HiddenState / NodeGatedHiddenState (graphML.py:3540-3681, 3857-4031) for long sequences:
+
+        z_t = f_t * z_{t-1} + i_t * sigma(A(S) x_t),     i_t = sigmoid(I(S) x_t),  f_t = sigmoid(F(S) x_t)
+
+    The gates are graph filters of the input (not of the previous state), so nothing in a step waits for the one before it but the recurrence
+    itself.  gate = 'element' (one gate per feature and node) or 'node' (one per node).  Parameters ``aWeights [H,E,K,F]``, ``xBias [H,1]`` and the
+    gates' filters ``inputGate`` / ``forgetGate``.  forward(x [B,T,F,N], z0 [B,H,N][, lengths]) -> (z [B,T,H,N], z_T [B,1,1,H,N]), as the other
+    hidden states."""
+
+    def __init__(self, F, H, K, nonlinearity=torch.tanh, E=1, bias=True, gate='element'):
+        super().__init__()
+        assert gate in ('element', 'node')
+        self.F = F
+        self.H = H
+        self.K = K
+        self.E = E
+        self.S = None
+        self._gso = None
+        self.bias = bias
+        self.sigma = nonlinearity
+        self.gate = gate
+        self.aWeights = nn.parameter.Parameter(torch.Tensor(H, E, K, F))
+        if self.bias:
+            self.xBias = nn.parameter.Parameter(torch.Tensor(H, 1))
+        else:
+            self.register_parameter('xBias', None)
+        width = H if gate == 'element' else 1
+        self.inputGate = GraphFilter(F, width, K, E, bias)
+        self.forgetGate = GraphFilter(F, width, K, E, bias)
+        self.reset_parameters()
+
+    def reset_parameters(self):
+        stdv = 1. / math.sqrt(self.F * self.K)
+        self.aWeights.data.uniform_(-stdv, stdv)
+        if self.bias:
+            self.xBias.data.uniform_(-stdv, stdv)
+
+    def addGSO(self, S):
+        if sp.issparse(S) or isinstance(S, (list, tuple)):
+            S = SparseGSO.from_any(S)
+        assert len(S.shape) == 3 and S.shape[0] == self.E
+        self.N = S.shape[1]
+        assert S.shape[2] == self.N
+        self.S = S
+        self._gso = SparseGSO.from_any(S)
+        self.inputGate.addGSO(self._gso)
+        self.forgetGate.addGSO(self._gso)
+
+    def forward(self, x, z0, lengths=None):
+        assert self._gso is not None
+        assert len(x.shape) == 4 and x.shape[2] == self.F
+        B, T, N = x.shape[0], x.shape[1], x.shape[3]
+        assert z0 is None or (len(z0.shape) == 3 and z0.shape[0] == B and z0.shape[1] == self.H and z0.shape[2] == N)
+        flat = x.reshape(B * T, self.F, N)
+        i = torch.sigmoid(self.inputGate(flat)).reshape(B, T, -1, N)
+        f = torch.sigmoid(self.forgetGate(flat)).reshape(B, T, -1, N)
+        z, zT = LinearGRNN(self.aWeights, self._gso, x, z0, self.sigma, i, f, xBias=self.xBias, lengths=lengths)
+        return z, zT.unsqueeze(1).unsqueeze(1)
+
+    def extra_repr(self):
+        reprString = "in_features=%d, hidden_features=%d, " % (self.F, self.H) + "filter_taps=%d, " % (self.K) + \
+                     "edge_features=%d, " % (self.E) + "bias=%s, " % (self.bias) + "nonlinearity=%s, " % (self.sigma) + "gate=%s, " % (self.gate)
         reprString += "GSO stored" if self.S is not None else "no GSO stored"
         return reprString
 
