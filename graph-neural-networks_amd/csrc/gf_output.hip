@@ -21,6 +21,7 @@ namespace {
 
 constexpr int kThr = 256;
 constexpr int kTopMax = 64;
+constexpr int kPackMax = 64;       // rows of up to so many outputs are packed into waves
 constexpr int kMaxNV = 4;          // 16-byte groups per thread and tile: 4 / 8 / 2 take 162 / 189 / 177 us for 4096 x 50001 bf16 with 8 alternatives
 constexpr int kCand = 1024;        // candidates that are ranked in LDS; more (heavy ties) take the extraction loop
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
@@ -610,6 +611,109 @@ __global__ __launch_bounds__(kThr) void distill_bwd_kernel(const D* __restrict__
     }
 }
 
+// ---- few outputs (V <= 64): G = 8 .. 64 lanes per row, one output per lane, 64 / G rows per wave ----------------------------------
+// A workgroup per row would be idle but for V of its 256 threads; with the rows packed, 1M rows of 5 classes move at the memory's rate.
+template <int G> struct Pack {
+    int i;                         // output
+    int64_t r;                     // row (clamped to the last one: lanes behind it compute on it and store nothing)
+    bool row_on, on;
+    __device__ __forceinline__ Pack(int64_t R, int V) {
+        const int lane = threadIdx.x & 63;
+        i = lane % G;
+        const int64_t q = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * (64 / G) + lane / G;
+        row_on = q < R;
+        r = row_on ? q : R - 1;
+        on = row_on && i < V;
+    }
+};
+template <int G> __device__ __forceinline__ float pack_max(float v) {
+#pragma unroll
+    for (int o = G / 2; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
+    return v;
+}
+template <int G> __device__ __forceinline__ float pack_sum(float v) {
+#pragma unroll
+    for (int o = G / 2; o; o >>= 1) v += __shfl_xor(v, o);
+    return v;
+}
+
+template <typename D, int G>
+__global__ __launch_bounds__(kThr) void token_pack_kernel(const D* __restrict__ logits, int64_t row_stride, int64_t R, int V, float c, int top, TokenOut ans) {
+    const Pack<G> p(R, V);
+    const D* row = logits + p.r * row_stride;
+    const float x = p.i < V ? gf_to_f<D>(row[p.i]) : -INFINITY;
+    const float m = pack_max<G>(x), ref = m == -INFINITY ? 0.f : m;
+    const float y = (x - ref) * (c * kLog2e), e = exp2_fast(y);
+    const float s = pack_sum<G>(e), t = pack_sum<G>(e * fmaxf(y, -3e38f)) * kLn2;
+    float ls = 0.f;
+    if (p.i == 0 && p.row_on) answer_row<D>(ans, p.r, row, V, c, m, s, t, ls);
+    if (top) {
+        ls = __shfl(ls, (threadIdx.x & 63) / G * G);
+        const unsigned o = ord32(x);
+        int rank = 0;
+        for (int j = 0; j < V; ++j) {
+            const unsigned oj = __shfl(o, (threadIdx.x & 63) / G * G + j);
+            rank += oj > o || (oj == o && j < p.i);
+        }
+        if (p.on && rank < top) answer_top(ans, p.r * top + rank, make_key(x, p.i), c, m, ls);
+    }
+}
+
+template <typename D, int G>
+__global__ __launch_bounds__(kThr) void token_pack_bwd_kernel(const D* __restrict__ logits, int64_t row_stride, const int64_t* __restrict__ tokens, float c,
+                                                              int64_t ignore_index, const float* __restrict__ stats, const int64_t* __restrict__ top_tokens,
+                                                              int top, const float* __restrict__ dlogp, const float* __restrict__ dentropy,
+                                                              const float* __restrict__ dtop, D* __restrict__ dlogits, int64_t R, int V) {
+    const Pack<G> p(R, V);
+    const float x = p.i < V ? gf_to_f<D>(logits[p.r * row_stride + p.i]) : 0.f;
+    const float m = stats[p.r * 3], ls = stats[p.r * 3 + 1], H = stats[p.r * 3 + 2];
+    const int64_t tok = tokens[p.r];
+    const bool empty = m == -INFINITY && ls == 0.f;
+    float w = 0.f;                                              // my output's own weight
+    if (dtop)
+        for (int k = 0; k < top; ++k) w += top_tokens[p.r * top + k] == p.i ? dtop[p.r * top + k] : 0.f;
+    if (dlogp && tok != ignore_index) {
+        const float g = dlogp[p.r];
+        if (tok < 0 || tok >= V) w = g != 0.f ? NAN : w;        // its log probability is NaN
+        else if (tok == p.i) w += g;
+    }
+    if (empty) w = 0.f;
+    const float A = pack_sum<G>(p.i < V ? w : 0.f), gH = (dentropy && !empty) ? dentropy[p.r] : 0.f;
+    const float lp = (x - m) * c - ls, q = exp2_fast(lp * kLog2e);
+    const float d = ((A == 0.f && gH == 0.f) || q == 0.f) ? 0.f : -c * q * fmaf(gH, lp + H, A);
+    if (p.on) dlogits[p.r * V + p.i] = gf_from_f<D>(w != 0.f ? d + c * w : d);
+}
+
+template <typename D, int G>
+__global__ __launch_bounds__(kThr) void distill_pack_kernel(const D* __restrict__ logits, int64_t row_stride, int64_t R, int V, float c,
+                                                            const int64_t* __restrict__ named, int K, Parts out) {
+    const Pack<G> p(R, V);
+    float x = p.i < V ? gf_to_f<D>(logits[p.r * row_stride + p.i]) : -INFINITY;
+    if (named)
+        for (int k = 0; k < K; ++k)
+            if (named[p.r * K + k] == p.i) x = -INFINITY;
+    const float m = pack_max<G>(x), ref = m == -INFINITY ? 0.f : m;
+    const float s = pack_sum<G>(exp2_fast((x - ref) * (c * kLog2e)));
+    if (p.i == 0 && p.row_on) {
+        out.m[p.r] = m;
+        out.s[p.r] = s;
+    }
+}
+
+template <typename D, int G>
+__global__ __launch_bounds__(kThr) void distill_pack_bwd_kernel(const D* __restrict__ logits, int64_t row_stride, const int64_t* __restrict__ indices,
+                                                                const float* __restrict__ probs, const float* __restrict__ stats, float c,
+                                                                const float* __restrict__ dloss, D* __restrict__ dlogits, int64_t R, int V, int K) {
+    const Pack<G> p(R, V);
+    const float x = p.i < V ? gf_to_f<D>(logits[p.r * row_stride + p.i]) : 0.f;
+    const float m = stats[p.r * 3], ls = stats[p.r * 3 + 1], g = c * dloss[p.r], w = g * stats[p.r * 3 + 2];
+    const bool none = g == 0.f || w == 0.f || (m == -INFINITY && ls == -INFINITY);
+    float d = none ? 0.f : w * exp2_fast(((x - m) * c - ls) * kLog2e);
+    for (int k = 0; k < K; ++k)
+        if (indices[p.r * K + k] == p.i) d = g == 0.f ? 0.f : g * probs[p.r * K + k];
+    if (p.on) dlogits[p.r * V + p.i] = gf_from_f<D>(d);
+}
+
 // ---- host ------------------------------------------------------------------------------------------------------------------
 // groups (16-byte vectors) per thread of a tile: up to kMaxNV once that gives the chip enough workgroups
 template <typename D> int pick_nv(int64_t R, int64_t V) {
@@ -635,6 +739,15 @@ Parts make_parts(void* ws, int64_t R, int64_t tiles, int top) {
     p.t = p.s + R * tiles;
     return p;
 }
+
+// f(lanes per row) for V <= 64; grid of packed rows
+template <typename F> int by_pack(int V, F&& f) {
+    if (V <= 8) return f(std::integral_constant<int, 8>());
+    if (V <= 16) return f(std::integral_constant<int, 16>());
+    if (V <= 32) return f(std::integral_constant<int, 32>());
+    return f(std::integral_constant<int, 64>());
+}
+dim3 pack_grid(int64_t R, int G) { return dim3((unsigned)((R + 4 * (64 / G) - 1) / (4 * (64 / G)))); }
 
 template <typename D, bool TOP, bool ENT, bool MASK, bool ONE>
 int run_tiles(const void* logits, int64_t row_stride, int64_t R, int V, int nv, int tiles, float c, int top, const int64_t* indices, int K,
@@ -670,9 +783,16 @@ template <typename D> void bwd_tiles(int64_t R, int64_t V, int& tiles, int& grou
 template <typename D>
 int token_forward_t(const void* logits, int64_t row_stride, const int64_t* tokens, float c, int64_t ignore, float* logp, float* entropy, float* top_logp,
                     int64_t* top_tokens, int top, float* stats, void* ws, int64_t R, int V, hipStream_t st) {
+    const TokenOut a{tokens, ignore, logp, entropy, top_logp, top_tokens, stats};
+    if (V <= kPackMax)
+        return by_pack(V, [&](auto g) -> int {
+            constexpr int G = decltype(g)::value;
+            token_pack_kernel<D, G><<<pack_grid(R, G), kThr, 0, st>>>(static_cast<const D*>(logits), row_stride, R, V, c, top, a);
+            GF_LAUNCH_CHECK("token_pack_kernel");
+            return GF_OK;
+        });
     const int nv = pick_nv<D>(R, V), tiles = (int)tiles_of<D>(V, nv);
     const Parts p = make_parts(ws, R, tiles, top);
-    const TokenOut a{tokens, ignore, logp, entropy, top_logp, top_tokens, stats};
     if (tiles == 1)
         return top ? run_tiles<D, true, true, false, true>(logits, row_stride, R, V, nv, 1, c, top, nullptr, 0, p, a, st)
                    : run_tiles<D, false, true, false, true>(logits, row_stride, R, V, nv, 1, c, 0, nullptr, 0, p, a, st);
@@ -687,6 +807,14 @@ int token_forward_t(const void* logits, int64_t row_stride, const int64_t* token
 template <typename D>
 int token_backward_t(const void* logits, int64_t row_stride, const int64_t* tokens, float c, int64_t ignore, const float* stats, const int64_t* top_tokens,
                      int top, const float* dlogp, const float* dentropy, const float* dtop, void* dlogits, int64_t R, int V, hipStream_t st) {
+    if (V <= kPackMax)
+        return by_pack(V, [&](auto g) -> int {
+            constexpr int G = decltype(g)::value;
+            token_pack_bwd_kernel<D, G><<<pack_grid(R, G), kThr, 0, st>>>(static_cast<const D*>(logits), row_stride, tokens, c, ignore, stats, top_tokens, top,
+                                                                          dlogp, dentropy, dtop, static_cast<D*>(dlogits), R, V);
+            GF_LAUNCH_CHECK("token_pack_bwd_kernel");
+            return GF_OK;
+        });
     int tiles, groups;
     bwd_tiles<D>(R, V, tiles, groups);
     token_bwd_kernel<D><<<dim3((unsigned)(R * tiles)), kThr, 0, st>>>(static_cast<const D*>(logits), row_stride, tokens, c, ignore, stats, top_tokens, top,
@@ -698,10 +826,18 @@ int token_backward_t(const void* logits, int64_t row_stride, const int64_t* toke
 template <typename D>
 int distill_forward_t(const void* logits, int64_t row_stride, const int64_t* indices, const float* values, float c, int tail, float* loss, float* stats,
                       float* probs, void* ws, int64_t R, int V, int K, hipStream_t st) {
-    const int nv = pick_nv<D>(R, V), tiles = (int)tiles_of<D>(V, nv);
+    const bool pack = V <= kPackMax;
+    const int nv = pick_nv<D>(R, V), tiles = pack ? 1 : (int)tiles_of<D>(V, nv);
     const Parts p = make_parts(ws, R, tiles, 0);
     const TokenOut none{};
-    const int rc = tail ? run_tiles<D, false, false, true, false>(logits, row_stride, R, V, nv, tiles, c, 0, indices, K, p, none, st)
+    const int rc = pack ? by_pack(V, [&](auto g) -> int {
+                              constexpr int G = decltype(g)::value;
+                              distill_pack_kernel<D, G><<<pack_grid(R, G), kThr, 0, st>>>(static_cast<const D*>(logits), row_stride, R, V, c,
+                                                                                          tail ? indices : nullptr, K, p);
+                              GF_LAUNCH_CHECK("distill_pack_kernel");
+                              return GF_OK;
+                          })
+                   : tail ? run_tiles<D, false, false, true, false>(logits, row_stride, R, V, nv, tiles, c, 0, indices, K, p, none, st)
                         : run_tiles<D, false, false, false, false>(logits, row_stride, R, V, nv, tiles, c, 0, nullptr, 0, p, none, st);
     if (rc != GF_OK) return rc;
     distill_finish_kernel<D><<<dim3((unsigned)((R + 3) / 4)), kThr, 0, st>>>(static_cast<const D*>(logits), row_stride, indices, values, c, tail, p, tiles,
@@ -713,6 +849,14 @@ int distill_forward_t(const void* logits, int64_t row_stride, const int64_t* ind
 template <typename D>
 int distill_backward_t(const void* logits, int64_t row_stride, const int64_t* indices, const float* probs, const float* stats, float c,
                        const float* dloss, void* dlogits, int64_t R, int V, int K, hipStream_t st) {
+    if (V <= kPackMax)
+        return by_pack(V, [&](auto g) -> int {
+            constexpr int G = decltype(g)::value;
+            distill_pack_bwd_kernel<D, G><<<pack_grid(R, G), kThr, 0, st>>>(static_cast<const D*>(logits), row_stride, indices, probs, stats, c, dloss,
+                                                                            static_cast<D*>(dlogits), R, V, K);
+            GF_LAUNCH_CHECK("distill_pack_bwd_kernel");
+            return GF_OK;
+        });
     int tiles, groups;
     bwd_tiles<D>(R, V, tiles, groups);
     distill_bwd_kernel<D><<<dim3((unsigned)(R * tiles)), kThr, 0, st>>>(static_cast<const D*>(logits), row_stride, indices, probs, stats, c, dloss,
