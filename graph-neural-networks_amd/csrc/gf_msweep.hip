@@ -917,7 +917,15 @@ int gf_msweep_launch(const gf_csr_dev& m, const float* Xin, float* Xtaps, int64_
 #undef GF_MS_P
 #undef GF_MS
 #undef GF_MSH
-    GF_HIP(lerr);
+    if (chained && lerr != hipSuccess) {
+        // The runtime has no cooperative queue to give (another process of this GPU holds the only one): nothing was launched.  The process goes on
+        // with one launch per hop -- the same bits -- and the callers run this chain that way.
+        (void)hipGetLastError();
+        if (!g_fuse_off.exchange(1))
+            fprintf(stderr, "gfhip: no cooperative launch for a fused K-hop chain (%s); the chain runs one launch per hop from here on\n", hipGetErrorString(lerr));
+        gf_set_error("cooperative launch of spmm_msweep_kernel: %s", hipGetErrorString(lerr));
+        return GF_ERR_UNSUPPORTED;
+    }
     GF_LAUNCH_CHECK("spmm_msweep_kernel");
     if (chained && !a_nostore && src_mask == 0xffffffffu) {
         hipLaunchKernelGGL(spmm_msweep_repair_kernel, dim3((unsigned)(B < 512 ? B : 512)), dim3(512), 0, st, gate + kMsCensusWord, m.rowptr, m.col, m.val, m.rowid,

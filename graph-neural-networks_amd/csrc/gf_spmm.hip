@@ -578,8 +578,8 @@ extern "C" int gf_khop(const gf_plan* const* plans, int32_t E, int32_t op, float
         const gf_csr_dev& m = plans[e]->mat[op];
         if (K > 2 && g_tune.spmm_fuse && gf_hop_uses_msweep(plans[e], op, B, W) && gf_msweep_fusion_allowed()) {
             const int rc = gf_msweep_launch(m, Z, Z + (int64_t)(1 + e * (K - 1)) * tap, tap, K - 1, plans[e]->n, B, W, gf_stream(stream));
-            if (rc != GF_OK) return rc;
-            continue;
+            if (rc == GF_OK) continue;
+            if (rc != GF_ERR_UNSUPPORTED) return rc;            // (no cooperative launch to be had: one launch per hop)
         }
         for (int k = 1; k < K; ++k) {
             const float* src = (k == 1) ? Z : Z + (int64_t)(1 + e * (K - 1) + (k - 2)) * tap;

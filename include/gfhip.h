@@ -254,7 +254,8 @@ int gf_spmm_hop_kernel(const gf_plan* plan, int32_t op, int32_t B, int32_t W);
  * 8 XCCs, all resident); a launch whose census fails, or that runs into its time limit, stores nothing, and the repair kernel queued behind it
  * recomputes the chain with the same bits -- no trap, no wrong result, no host synchronisation.  flags: bit 0 = a census failed, bit 1 = a
  * time limit expired (since the process started); fusion_on = 0 once that has been seen by the host (gf_khop then runs one launch per hop)
- * or when GFHIP_MSWEEP_FUSE=0 is set in the environment. */
+ * or when GFHIP_MSWEEP_FUSE=0 is set in the environment, or when the runtime refused a cooperative launch (another process on this GPU
+ * holds the cooperative queue). */
 int gf_msweep_status(uint32_t* flags, int32_t* fusion_on);
 int gf_time_khop(const gf_plan* const* plans, int32_t E, int32_t op, float* Z, int32_t B, int32_t W, int32_t K, int32_t iters,
                  void* stream, float* avg_ms);   /* the same for one gf_khop call (the K-1 hops of every edge feature on a tap stack) */

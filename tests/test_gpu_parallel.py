@@ -189,3 +189,41 @@ def test_fused_chains_of_two_processes_on_one_gpu_do_not_trap_hang_or_differ():
         assert same and equal_ref, (rank, same, equal_ref, flags, fusion_on)
     import warnings
     warnings.warn(f"two processes, one GPU: status flags per rank {[ret[r][2] for r in range(world)]}, fusion still on {[ret[r][3] for r in range(world)]}")
+
+
+def _chain_child():
+    """A fused chain's results in a process of its own, beside the parent's (which holds the cooperative queue)."""
+    import scipy.sparse as sp
+    from alegnn_amd import _lib
+    from alegnn_amd.gso import SparseGSO
+    n, B, K, W = 60000, 8, 4, 32
+    rng = np.random.RandomState(7)
+    r = np.repeat(np.arange(n), 4)
+    A = sp.csr_matrix((np.full(r.size, 0.125), (r, rng.randint(0, n, size=r.size))), shape=(n, n))
+    A.sum_duplicates()
+    gso = SparseGSO([A])
+    dev = torch.device("cuda:0")
+    plans, L = gso.plans(dev), _lib.lib()
+    st = torch.cuda.current_stream().cuda_stream
+    Z = torch.empty((K, B, n, W), device=dev)
+    Z[0] = torch.linspace(-1, 1, B * n * W, device=dev).view(B, n, W)
+    Z[1:] = float("nan")
+    for _ in range(2):                                  # the first call may find no cooperative queue, the second starts without one
+        _lib.check(L.gf_khop(plans, 1, 0, Z.data_ptr(), B, W, K, st))
+    torch.cuda.synchronize()
+    return Z
+
+
+def _chain_child_main(rank, ret):
+    Z = _chain_child()
+    ret["sums"] = [float(Z[k].double().sum()) for k in range(4)]
+    ret["probe"] = Z[:, :, ::997].cpu()
+
+
+def test_a_chain_beside_a_process_that_holds_the_cooperative_queue():
+    """Some driver versions give the cooperative queue to one process per GPU: the other process's chains run one launch per hop, with the same bits."""
+    here = _chain_child()
+    ret = mp.get_context("spawn").Manager().dict()
+    mp.spawn(_chain_child_main, args=(ret,), nprocs=1, join=True)
+    assert torch.equal(ret["probe"], here[:, :, ::997].cpu())
+    assert ret["sums"] == [float(here[k].double().sum()) for k in range(4)]
