@@ -8,8 +8,6 @@ alegnn/modules/evaluation.py:58-71); here an answer is a probability with its al
 can be trained on."""
 from __future__ import annotations
 
-import math
-
 import torch
 
 from . import _lib
@@ -28,6 +26,7 @@ def _rows(who, logits, dim):
         logits = logits.movedim(dim, -1)
     V = logits.shape[-1]
     assert V > 0, f"{who}: logits have shape {tuple(logits.shape)}: no outputs to choose from"
+    assert V < 2 ** 31 - 2 ** 16, f"{who}: {V} outputs (fewer than 2^31 - 2^16 are supported)"
     x = logits if logits.dim() == 2 else logits.reshape(-1, V)
     if V > 1 and x.stride(1) != 1:
         x = x.contiguous()
@@ -36,8 +35,8 @@ def _rows(who, logits, dim):
 
 def _check_temperature(who, temperature):
     temperature = float(temperature)
-    if not (temperature > 0.0 and math.isfinite(temperature)):
-        raise ValueError(f"alegnn_amd.{who}: temperature {temperature} (want a positive number)")
+    if not 1e-30 <= temperature <= 1e30:
+        raise ValueError(f"alegnn_amd.{who}: temperature {temperature} (want a number between 1e-30 and 1e30)")
     return temperature
 
 

@@ -145,6 +145,7 @@ def linear_recurrence(u, q_check, q_hat=None, z0=None, lengths=None):
     who = "linear_recurrence"
     assert u.dim() == 4, f"{who}: u has shape {tuple(u.shape)}, want [B, T, H, N]"
     _require_cuda(who, "u", u, _FLOATS)
+    assert max(u.shape) <= 2 ** 31 - 2 ** 17, f"{who}: u has shape {tuple(u.shape)}: a side over 2^31 - 2^17"
     kinds = [0, 0, 0 if q_hat is None else 1]
     for i, name, q in ((0, "q_check", q_check), (1, "q_hat", q_hat)):
         if q is not None:

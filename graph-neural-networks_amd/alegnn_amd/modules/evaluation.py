@@ -45,17 +45,18 @@ def evaluateSingleNode(model, data, **kwargs):
 
 
 def predictTop(model, data, samplesType='test', top=5, temperature=1.0, batchSize=None):
-    """What the model's architecture, as it stands, answers on a split of a classification data set (outputs B x classes, labels B): a dict of
-    'logProb' [B] (of the true class), 'entropy' [B], and the `top` best classes per sample 'topLogProb' / 'topClasses' [B, top], under
+    """What the model's architecture, as it stands, answers on a split of a classification data set (outputs B x classes [x nodes], labels B [x nodes]):
+    a dict of 'logProb' [B] (of the true class), 'entropy' [B], and the `top` best classes per sample 'topLogProb' / 'topClasses' [B, top], under
     softmax(output / temperature).  (topClasses, topLogProb) of the training split is what Trainer takes as teacherTop."""
     x, y = data.getSamples(samplesType)
     n = x.shape[0]
+    assert n > 0 and (batchSize is None or batchSize > 0)
     step = n if batchSize is None else int(batchSize)
     parts = []
     with torch.no_grad():
         for b in range(0, n, step):
             out = model.archit(x[b:b + step].to(model.device))
-            labels = y[b:b + step].to(model.device).to(torch.int64).reshape(out.shape[0])
-            parts.append(token_log_probs(out, labels, top=min(int(top), out.shape[1]), temperature=temperature))
+            labels = y[b:b + step].to(model.device).to(torch.int64).reshape(out.shape[:1] + out.shape[2:])
+            parts.append(token_log_probs(out, labels, top=min(int(top), out.shape[1]), temperature=temperature, dim=1))
     names = ('logProb', 'entropy', 'topLogProb', 'topClasses')
     return {k: None if parts[0][i] is None else torch.cat([p[i] for p in parts]) for i, k in enumerate(names)}

@@ -764,12 +764,28 @@ int run_tiles(const void* logits, int64_t row_stride, int64_t R, int V, int nv, 
 int check_rows(const char* who, int64_t R, int64_t V, int64_t row_stride, int dtype, float temperature) {
     GF_REQUIRE_ARG(gf_dtype_ok(dtype), "%s: dtype %d", who, dtype);
     GF_REQUIRE_SHAPE(R > 0 && V > 0 && row_stride >= 0, "%s: bad shape R=%lld V=%lld row stride %lld", who, (long long)R, (long long)V, (long long)row_stride);
-    GF_REQUIRE_ARG(temperature > 0.f && temperature < INFINITY, "%s: temperature %g", who, (double)temperature);
-    // one workgroup per (row, tile of at least 1024 elements): the launch grid is 32 bits wide
-    GF_REQUIRE_SHAPE(V < (1ll << 31) - 64 && R < (1ll << 31) && (double)R * ((double)V / 1024.0 + 2.0) < 2147483000.0, "%s: R=%lld rows of V=%lld are too many", who,
-                     (long long)R, (long long)V);
+    // (1 / temperature and the exponents' scale stay finite and normal)
+    GF_REQUIRE_ARG(temperature >= 1e-30f && temperature <= 1e30f, "%s: temperature %g (1e-30 .. 1e30)", who, (double)temperature);
+    GF_REQUIRE_SHAPE(V < (1ll << 31) - (1 << 16), "%s: rows of V=%lld outputs", who, (long long)V);
     return GF_OK;
 }
+
+// rows per launch: one workgroup of 256 threads per (row, tile of at least 1024 elements), and a launch's threads are counted in 32 bits
+int64_t rows_per_launch(int64_t V) {
+    const int64_t n = (1ll << 23) / (V / 1024 + 2);
+    return n < 1 ? 1 : n;
+}
+template <typename F> int in_batches(int64_t R, int64_t V, F&& f) {   // f(first row, rows)
+    const int64_t step = rows_per_launch(V);
+    for (int64_t r = 0; r < R; r += step) {
+        const int rc = f(r, R - r < step ? R - r : step);
+        if (rc != GF_OK) return rc;
+    }
+    return GF_OK;
+}
+const char* row_at(const void* p, int64_t r, int64_t stride, int dtype) { return static_cast<const char*>(p) + r * stride * (int64_t)gf_dtype_bytes(dtype); }
+char* row_at(void* p, int64_t r, int64_t stride, int dtype) { return static_cast<char*>(p) + r * stride * (int64_t)gf_dtype_bytes(dtype); }
+template <typename T> T* at(T* p, int64_t i) { return p ? p + i : nullptr; }
 
 // tiles of a gradient kernel: 16 KiB of logits per workgroup where that gives enough workgroups, fewer otherwise
 template <typename D> void bwd_tiles(int64_t R, int64_t V, int& tiles, int& groups) {
@@ -873,9 +889,20 @@ template <typename F> int by_dtype(int dtype, F&& f) {
 
 }  // namespace
 
+// scratch of the largest batch (the last, shorter one may be cut into smaller tiles: never into more than this bound)
+static size_t batch_bytes(int64_t R, int64_t V, int top, int dtype) {
+    const int64_t step = rows_per_launch(V), full = R < step ? R : step, last = R % step;
+    size_t b = parts_bytes(full, tiles_for(full, V, dtype), top);
+    if (R > step && last) {
+        const size_t c = parts_bytes(last, tiles_for(last, V, dtype), top);
+        b = b > c ? b : c;
+    }
+    return b;
+}
+
 extern "C" size_t gf_token_logp_workspace_bytes(int64_t R, int32_t V, int32_t top, int32_t dtype) {
     if (R <= 0 || V <= 0 || top < 0 || !gf_dtype_ok(dtype)) return 0;
-    return parts_bytes(R, tiles_for(R, V, dtype), top);
+    return batch_bytes(R, V, top, dtype);
 }
 
 extern "C" int gf_token_logp_forward(const void* logits, int64_t row_stride, const int64_t* tokens, float temperature, int64_t ignore_index, float* logp,
@@ -889,8 +916,11 @@ extern "C" int gf_token_logp_forward(const void* logits, int64_t row_stride, con
     GF_REQUIRE_ARG(workspace && workspace_bytes >= need && reinterpret_cast<uintptr_t>(workspace) % 8 == 0,
                    "gf_token_logp_forward: workspace of %zu bytes, needs %zu, 8-byte aligned", workspace_bytes, need);
     return by_dtype(dtype, [&](auto d) -> int {
-        return token_forward_t<decltype(d)>(logits, row_stride, tokens, 1.f / temperature, ignore_index, logp, entropy, top_logp, top_tokens, top, stats,
-                                            workspace, R, V, gf_stream(stream));
+        return in_batches(R, V, [&](int64_t r, int64_t n) {
+            return token_forward_t<decltype(d)>(row_at(logits, r, row_stride, dtype), row_stride, tokens + r, 1.f / temperature, ignore_index, logp + r,
+                                                at(entropy, r), at(top_logp, r * top), at(top_tokens, r * top), top, at(stats, r * 3), workspace, n, V,
+                                                gf_stream(stream));
+        });
     });
 }
 
@@ -902,14 +932,17 @@ extern "C" int gf_token_logp_backward(const void* logits, int64_t row_stride, co
     GF_REQUIRE_SHAPE(top >= 0 && top <= kTopMax && top <= V, "gf_token_logp_backward: top=%d (0..min(V, %d))", top, kTopMax);
     GF_REQUIRE_ARG(logits && tokens && stats && dlogits && (top == 0 || top_tokens), "gf_token_logp_backward: NULL tensor");
     return by_dtype(dtype, [&](auto d) -> int {
-        return token_backward_t<decltype(d)>(logits, row_stride, tokens, 1.f / temperature, ignore_index, stats, top_tokens, top, dlogp, dentropy, dtop,
-                                             dlogits, R, V, gf_stream(stream));
+        return in_batches(R, V, [&](int64_t r, int64_t n) {
+            return token_backward_t<decltype(d)>(row_at(logits, r, row_stride, dtype), row_stride, tokens + r, 1.f / temperature, ignore_index, stats + r * 3,
+                                                 at(top_tokens, r * top), top, at(dlogp, r), at(dentropy, r), at(dtop, r * top),
+                                                 row_at(dlogits, r, V, dtype), n, V, gf_stream(stream));
+        });
     });
 }
 
 extern "C" size_t gf_distill_top_workspace_bytes(int64_t R, int32_t V, int32_t K, int32_t dtype) {
     if (R <= 0 || V <= 0 || K <= 0 || !gf_dtype_ok(dtype)) return 0;
-    return parts_bytes(R, tiles_for(R, V, dtype), 0);
+    return batch_bytes(R, V, 0, dtype);
 }
 
 extern "C" int gf_distill_top_forward(const void* logits, int64_t row_stride, const int64_t* indices, const float* values, float temperature, int32_t tail,
@@ -923,8 +956,10 @@ extern "C" int gf_distill_top_forward(const void* logits, int64_t row_stride, co
     GF_REQUIRE_ARG(workspace && workspace_bytes >= need && reinterpret_cast<uintptr_t>(workspace) % 8 == 0,
                    "gf_distill_top_forward: workspace of %zu bytes, needs %zu, 8-byte aligned", workspace_bytes, need);
     return by_dtype(dtype, [&](auto d) -> int {
-        return distill_forward_t<decltype(d)>(logits, row_stride, indices, values, 1.f / temperature, tail, loss, stats, probs, workspace, R, V, K,
-                                              gf_stream(stream));
+        return in_batches(R, V, [&](int64_t r, int64_t n) {
+            return distill_forward_t<decltype(d)>(row_at(logits, r, row_stride, dtype), row_stride, indices + r * K, values + r * K, 1.f / temperature, tail,
+                                                  loss + r, stats + r * 3, probs + r * K, workspace, n, V, K, gf_stream(stream));
+        });
     });
 }
 
@@ -937,6 +972,9 @@ extern "C" int gf_distill_top_backward(const void* logits, int64_t row_stride, c
     GF_REQUIRE_ARG(logits && indices && probs && stats && dloss && dlogits, "gf_distill_top_backward: NULL tensor");
     (void)tail;
     return by_dtype(dtype, [&](auto d) -> int {
-        return distill_backward_t<decltype(d)>(logits, row_stride, indices, probs, stats, 1.f / temperature, dloss, dlogits, R, V, K, gf_stream(stream));
+        return in_batches(R, V, [&](int64_t r, int64_t n) {
+            return distill_backward_t<decltype(d)>(row_at(logits, r, row_stride, dtype), row_stride, indices + r * K, probs + r * K, stats + r * 3,
+                                                   1.f / temperature, dloss + r, row_at(dlogits, r, V, dtype), n, V, K, gf_stream(stream));
+        });
     });
 }

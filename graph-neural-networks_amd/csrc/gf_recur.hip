@@ -622,6 +622,7 @@ int check_dims(const char* who, int B, int T, int H, int N, int dtype, int kc, i
     GF_REQUIRE_ARG((kc & ~7) == 0 && (kh & ~7) == 0, "%s: gate kinds %d, %d", who, kc, kh);
     GF_REQUIRE_SHAPE(B > 0 && T >= 0 && H > 0 && N > 0, "%s: bad shape B=%d T=%d H=%d N=%d", who, B, T, H, N);
     GF_REQUIRE_SHAPE((int64_t)H * N < (1ll << 30), "%s: H * N = %lld channels", who, (long long)H * N);
+    GF_REQUIRE_SHAPE(T <= INT32_MAX - (1 << 16), "%s: T = %d steps", who, T);                 // (a slab's end stays an int32)
     return GF_OK;
 }
 
@@ -759,7 +760,8 @@ extern "C" int gf_recurrence_forward(const void* u, const void* q_check, int32_t
                    workspace_bytes, agg_floats(d) * 4);
     GF_REQUIRE_ARG(s.V == 1 || (aligned(u, 4 * el) && aligned(q_check, 4 * el) && aligned(q_hat, 4 * el) && aligned(z, 4 * el)),
                    "gf_recurrence_forward: a tensor is not aligned to four elements");
-    GF_REQUIRE_SHAPE((int64_t)d.chunks * d.splits * B < (1ll << 31), "gf_recurrence_forward: too many workgroups (B=%d, H*N=%d)", B, d.C);
+    // (256 threads per workgroup, and a launch's threads are counted in 32 bits)
+    GF_REQUIRE_SHAPE((int64_t)d.chunks * d.splits * B < (1ll << 24), "gf_recurrence_forward: too many workgroups (B=%d, H*N=%d)", B, d.C);
     const Gate gc = make_gate(q_check, kind_check, T, H, N), gh = make_gate(q_hat, kind_hat, T, H, N);
     float* ws = static_cast<float*>(workspace);
     hipStream_t st = gf_stream(stream);
@@ -784,7 +786,7 @@ extern "C" int gf_recurrence_backward(const void* u, const void* q_check, int32_
     GF_REQUIRE_ARG(s.V == 1 || (aligned(u, 4 * el) && aligned(q_check, 4 * el) && aligned(q_hat, 4 * el) && aligned(dz, 4 * el) && aligned(du, 4 * el) &&
                                 aligned(dq_check, 4 * el) && aligned(dq_hat, 4 * el) && aligned(workspace, 16)),
                    "gf_recurrence_backward: a tensor is not aligned to four elements");
-    GF_REQUIRE_SHAPE((int64_t)d.chunks * d.splits * B < (1ll << 31), "gf_recurrence_backward: too many workgroups (B=%d, H*N=%d)", B, d.C);
+    GF_REQUIRE_SHAPE((int64_t)d.chunks * d.splits * B < (1ll << 24), "gf_recurrence_backward: too many workgroups (B=%d, H*N=%d)", B, d.C);
     const Gate gc = make_gate(q_check, kind_check, T, H, N), gh = make_gate(q_hat, kind_hat, T, H, N);
     float* ws = static_cast<float*>(workspace);
     hipStream_t st = gf_stream(stream);

@@ -274,7 +274,7 @@ enum { GF_GATE_N = 1, GF_GATE_H = 2, GF_GATE_B = 4 };
  * length are not read, leave the state as it is and give z = 0.  zT [B, H, N] fp32 is the last state.
  * checkpoints (gf_recurrence_checkpoint_floats, NULL = not kept): one fp32 state every few steps, what the backward pass recomputes the
  * states from.  Products of q_check over a few hundred steps must stay finite in fp32.
- * Tensors are aligned to four elements.  B >= 1, T >= 0, H N < 2^30. */
+ * Tensors are aligned to four elements.  B >= 1, T >= 0, H N < 2^30; B times the channel chunks (16 to 256 channels) < 2^24. */
 size_t gf_recurrence_checkpoint_floats(int32_t B, int32_t T, int32_t H, int32_t N, int32_t kind_check, int32_t has_hat, int32_t kind_hat);
 size_t gf_recurrence_workspace_bytes(int32_t B, int32_t T, int32_t H, int32_t N, int32_t kind_check, int32_t has_hat, int32_t kind_hat, int32_t backward);
 int gf_recurrence_forward(const void* u, const void* q_check, int32_t kind_check, const void* q_hat, int32_t kind_hat, const float* z0,
@@ -292,7 +292,8 @@ int gf_recurrence_backward(const void* u, const void* q_check, int32_t kind_chec
  *   lp = log softmax(logits / temperature);  logp [R] = lp[token], entropy [R] = -sum p lp (NULL = not wanted), top_tokens / top_logp
  *   [R, top]: the `top` largest logits of each row, largest first, equal ones in ascending index order (NaN counts as the largest).
  * stats [R, 3] fp32 (row maximum, log of the sum, entropy): what the backward pass needs.  -inf marks an output that is ruled out
- * (p = 0); a row of nothing else has logp = -inf, entropy 0 and gradient 0.  0 <= top <= min(V, 64).  No alignment is assumed. */
+ * (p = 0); a row of nothing else has logp = -inf, entropy 0 and gradient 0.  0 <= top <= min(V, 64), temperature 1e-30 .. 1e30.
+ * No alignment is assumed; the workspace is 8-byte aligned. */
 size_t gf_token_logp_workspace_bytes(int64_t R, int32_t V, int32_t top, int32_t dtype);
 int gf_token_logp_forward(const void* logits, int64_t row_stride, const int64_t* tokens, float temperature, int64_t ignore_index, float* logp,
                           float* entropy, float* top_logp, int64_t* top_tokens, int32_t top, float* stats, void* workspace, size_t workspace_bytes,

@@ -330,3 +330,30 @@ def test_more_than_two_to_the_31_elements():
     want, tol = ref.distill(xs, np.array([[5, V - 1]] * 4), np.zeros((4, 2)), 1.0, False, np.ones(4), half(torch.bfloat16))
     within(loss[rows], want["loss"], tol["loss"], "loss")
     within(dd[rows], want["dlogits"], tol["dlogits"], "dlogits")
+
+
+@pytest.mark.parametrize("V,dtype", [(5, "f32"), (70, "bf16")])
+def test_more_rows_than_one_launch_takes(V, dtype):
+    R = (1 << 22) + 1003                                            # launches hold 2^22 such rows
+    g = torch.Generator(device="cuda").manual_seed(V)
+    x = torch.empty((R, V), device="cuda").normal_(generator=g).to(DT[dtype])
+    tok = torch.randint(0, V, (R,), generator=g, device="cuda")
+    idx = torch.randint(0, V, (R, 2), generator=g, device="cuda")
+    val = torch.zeros((R, 2), device="cuda")
+    leaf = x.requires_grad_()
+    logp, ent, tl, ti = token_log_probs(leaf, tok, top=3)
+    d = torch.autograd.grad([logp, ent], leaf, [torch.ones_like(logp), torch.ones_like(ent)])[0]
+    loss = distill_top(leaf, idx, val)
+    dd = torch.autograd.grad(loss.sum(), leaf)[0]
+    rows = [0, (1 << 22) - 1, 1 << 22, (1 << 22) + 1, R - 1]
+    xs = x.detach()[rows].double().cpu().numpy()
+    one = np.ones(len(rows))
+    want, tol = ref.tokens(xs, tok[rows].cpu().numpy(), 3, 1.0, -100, one, one, None, half(DT[dtype]))
+    within(logp[rows], want["logp"], tol["logp"], "logp")
+    within(ent[rows], want["entropy"], tol["entropy"], "entropy")
+    within(tl[rows], want["top_logp"], tol["top_logp"], "top_logp")
+    assert np.array_equal(ti[rows].cpu().numpy(), want["top_tokens"])
+    within(d[rows], want["dlogits"], tol["dlogits"], "dlogits")
+    want, tol = ref.distill(xs, idx[rows].cpu().numpy(), val[rows].double().cpu().numpy(), 1.0, False, one, half(DT[dtype]))
+    within(loss[rows], want["loss"], tol["loss"], "loss")
+    within(dd[rows], want["dlogits"], tol["dlogits"], "dlogits")

@@ -26,6 +26,7 @@ def recurrence_args(**kw):
 @pytest.mark.parametrize("kw,code,word", [
     (dict(dtype=3), -2, b"dtype"), (dict(kc=8), -2, b"gate kinds"), (dict(kh=-1), -2, b"gate kinds"), (dict(B=0), -1, b"bad shape"),
     (dict(T=-1), -1, b"bad shape"), (dict(H=0), -1, b"bad shape"), (dict(N=-4), -1, b"bad shape"), (dict(H=1 << 15, N=1 << 15), -1, b"channels"),
+    (dict(T=(1 << 31) - 1, H=1, N=1), -1, b"steps"),
     (dict(u=None), -2, b"NULL"), (dict(qc=None), -2, b"NULL"), (dict(z=None), -2, b"NULL"), (dict(zT=None), -2, b"NULL"), (dict(u=68), -2, b"aligned"),
     (dict(qh=72), -2, b"aligned"), (dict(z=4), -2, b"aligned"), (dict(B=1, T=70000, N=4, ws=None, nb=0), -2, b"workspace"),
     (dict(B=(1 << 31) - 1, H=1 << 10, N=1 << 10), -1, b"too many"),
@@ -74,8 +75,8 @@ def token_args(**kw):
     (dict(temperature=0.0), -2, b"temperature"), (dict(temperature=-1.0), -2, b"temperature"), (dict(temperature=float("inf")), -2, b"temperature"),
     (dict(temperature=float("nan")), -2, b"temperature"), (dict(top=-1), -1, b"top"), (dict(top=11), -1, b"top"), (dict(top=65, V=100), -1, b"top"),
     (dict(x=None), -2, b"NULL"), (dict(tokens=None), -2, b"NULL"), (dict(logp=None), -2, b"NULL"), (dict(tl=None), -2, b"NULL"), (dict(ti=None), -2, b"NULL"),
-    (dict(ws=None), -2, b"workspace"), (dict(nb=8), -2, b"workspace"), (dict(ws=68), -2, b"workspace"), (dict(R=1 << 31), -1, b"too many"),
-    (dict(R=1 << 24, V=1 << 24), -1, b"too many"),
+    (dict(ws=None), -2, b"workspace"), (dict(nb=8), -2, b"workspace"), (dict(ws=68), -2, b"workspace"),
+    (dict(V=(1 << 31) - 1), -1, b"outputs"), (dict(temperature=1e-38), -2, b"temperature"),
 ])
 def test_token_forward_refuses(kw, code, word):
     L = _lib.lib()
