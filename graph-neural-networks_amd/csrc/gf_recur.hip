@@ -42,33 +42,42 @@ struct Dims {
     int32_t nck;                   // checkpoints per sequence
 };
 
-// The loads of a slab are straight-line code (addresses clamped to the last live step, values replaced afterwards): all of them are in
-// flight before the first one is waited for.  A gate without the node axis has one value for the thread's V channels (V > 1 only where they
-// share the feature); it is spread after the other loads have been issued.
-template <typename D, int V>
-__device__ __forceinline__ void load_gate(const Gate& g, int64_t at, const int (&t)[kL], gf_vec<D, V> (&raw)[kL]) {
-    const D* p = static_cast<const D*>(g.p) + at;
-    if (V > 1 && (g.kind & GF_GATE_N)) {
+// What a wave reads or writes of a tensor in a slab: `base` is the same for the whole wave (sequence, wave's first row), `off` is the lane's byte
+// offset in it (its row group's first row, its channel), so the address of step l is one scalar and one 32-bit vector register.
+struct Stream {
+    char* base;
+    int64_t step;                  // bytes per time step
+    uint32_t off;
+    int32_t row;                   // the lane's first row at ts = 0
+    __device__ __forceinline__ char* at(int t) const { return base + (int64_t)t * step + off; }             // t = ts + l
+};
+template <typename D> __device__ __forceinline__ Stream stream(const void* p, int64_t first, int wrow, int lrow, int st, int coff) {
+    Stream s;
+    s.base = const_cast<char*>(static_cast<const char*>(p)) + (first + (int64_t)wrow * st) * (int64_t)sizeof(D);
+    s.step = (int64_t)st * (int64_t)sizeof(D);
+    s.off = ((uint32_t)lrow * (uint32_t)st + (uint32_t)coff) * (uint32_t)sizeof(D);
+    s.row = wrow + lrow;
+    return s;
+}
+// The loads of a slab are straight-line code: all of them are in flight before the first one is waited for.  VEC: V elements per step, else one value
+// for the thread's V channels (a gate without the node axis; V > 1 only where they share the feature).  Rows behind the last step of the tensor
+// are clamped to the last live one (only in a tensor's last slab: the lane's address is then computed the long way).
+template <typename D, int V, bool VEC> __device__ __forceinline__ void load_one(const char* p, gf_vec<D, V>& raw) {
+    if constexpr (VEC) raw = *reinterpret_cast<const gf_vec<D, V>*>(p);
+    else raw.e[0] = *reinterpret_cast<const D*>(p);
+}
+template <typename D, int V, bool VEC>
+__device__ __forceinline__ void load_slab(const Stream& s, int ts, bool inside, int last, gf_vec<D, V> (&raw)[kL]) {
+    if (inside) {
 #pragma unroll
-        for (int l = 0; l < kL; ++l) raw[l] = *reinterpret_cast<const gf_vec<D, V>*>(p + (int64_t)t[l] * g.st);
+        for (int l = 0; l < kL; ++l) load_one<D, V, VEC>(s.at(ts + l), raw[l]);
     } else {
 #pragma unroll
-        for (int l = 0; l < kL; ++l) raw[l].e[0] = p[(int64_t)t[l] * g.st];
+        for (int l = 0; l < kL; ++l) load_one<D, V, VEC>(s.base + s.off + (int64_t)(min(ts + s.row + l, last) - s.row) * s.step, raw[l]);
     }
 }
-template <typename D, int V> __device__ __forceinline__ void spread_gate(const Gate& g, gf_vec<D, V> (&raw)[kL]) {
-    if (V > 1 && !(g.kind & GF_GATE_N)) {
-#pragma unroll
-        for (int l = 0; l < kL; ++l)
-#pragma unroll
-            for (int i = 1; i < V; ++i) raw[l].e[i] = raw[l].e[0];
-    }
-}
-template <typename D, int V>
-__device__ __forceinline__ void load_rows(const D* __restrict__ p, int64_t C, const int (&t)[kL], gf_vec<D, V> (&raw)[kL]) {
-#pragma unroll
-    for (int l = 0; l < kL; ++l) raw[l] = *reinterpret_cast<const gf_vec<D, V>*>(p + t[l] * C);
-}
+template <typename D, int V, bool VEC> __device__ __forceinline__ float pick(const gf_vec<D, V>& raw, int i) { return gf_to_f<D>(raw.e[VEC ? i : 0]); }
+
 __device__ __forceinline__ int gate_coff(const Gate& g, int c, int N) {
     if (g.kind == (GF_GATE_H | GF_GATE_N)) return c;
     if (g.kind == GF_GATE_N) return c % N;
@@ -83,15 +92,24 @@ struct Place {
     static constexpr int NW = WT == 1 ? 4 : WT;                 // waves of a workgroup
     static constexpr int CW = (WT == 1 ? NW * CX : CX) * V;     // channels of a workgroup
     static constexpr int SLAB = WT * GW * kL;
-    int lane, wave, cx, tg, c, b, split;
-    bool on;
+    int lane, wave, cx, tg, c, b, split, column;
+    bool on, work;                  // channel inside the row; (uniform) workgroup has work
     __device__ __forceinline__ Place(const Dims& d) {
         lane = threadIdx.x & 63;
-        wave = threadIdx.x >> 6;
+        wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
         cx = lane % CX;
         tg = (WT == 1 ? 0 : wave * GW) + lane / CX;
-        const unsigned blk = blockIdx.x;
+        unsigned blk = blockIdx.x;
+        if (d.splits > 1) {
+            // Workgroups go to the 8 XCDs in turn.  Long runs put all chunks of a (sequence, split) on one XCD: a chunk's row segments (128 bytes,
+            // starting at any multiple of V elements) share their cache lines with its neighbours' (65537 x 808 bf16: 291 -> 269 us).  Without splits
+            // there is work enough to stream, and sequences of unlike lengths are better spread over the XCDs (32 x 257 x 53824: 1361 / 1513 us).
+            const unsigned x = blk & 7u, k = blk >> 3;
+            blk = (x + 8u * (k / (unsigned)d.chunks)) * (unsigned)d.chunks + k % (unsigned)d.chunks;
+        }
         const unsigned chunk = blk % (unsigned)d.chunks, rest = blk / (unsigned)d.chunks;
+        work = rest < (unsigned)d.splits * (unsigned)d.B;
+        column = (int)chunk;
         split = (int)(rest % (unsigned)d.splits);
         b = (int)(rest / (unsigned)d.splits);
         c = (int)chunk * CW + (WT == 1 ? wave * CX : 0) * V + cx * V;
@@ -99,47 +117,57 @@ struct Place {
     }
 };
 
-// exclusive composition of the stretches before (FWD) / behind (!FWD) this thread's own, and of the whole slab
+// Rows of 16 lanes moved inside the vector unit (no LDS traffic): of x's rows (0, 1, 2, 3), lo16 = (0, 0, 2, 2), hi16 = (1, 1, 3, 3),
+// lo32 = (0, 1, 0, 1), hi32 = (2, 3, 2, 3).
+__device__ __forceinline__ float lo16(float x) { return __uint_as_float(__builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false)[0]); }
+__device__ __forceinline__ float hi16(float x) { return __uint_as_float(__builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false)[1]); }
+__device__ __forceinline__ float lo32(float x) { return __uint_as_float(__builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false)[0]); }
+__device__ __forceinline__ float hi32(float x) { return __uint_as_float(__builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false)[1]); }
+
+// exclusive composition of the stretches before (FWD) / behind (!FWD) this thread's own, and of the whole slab.  GW = 4: the wave's rows of 16
+// lanes are the stretches (pairs first, then the halves); WT > 1: the waves' compositions through LDS.
 template <int V, int WT, int GW, bool FWD>
 __device__ __forceinline__ void join(const float (&A)[V], const float (&S)[V], float (&Ae)[V], float (&Se)[V], float (&At)[V], float (&St)[V],
                                      int lane, int wave, float* lds) {
+    static_assert(GW == 1 || GW == 4, "a wave's stretches are its rows of 16 lanes, or one");
     constexpr int CX = 64 / GW;
-    float a[V], s[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) a[i] = A[i], s[i] = S[i];
-#pragma unroll
-    for (int off = CX; off < 64; off <<= 1) {
-        const bool take = FWD ? lane >= off : lane < 64 - off;
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const float ao = FWD ? __shfl_up(a[i], off) : __shfl_down(a[i], off);
-            const float so = FWD ? __shfl_up(s[i], off) : __shfl_down(s[i], off);
-            if (take) {
-                s[i] = fmaf(a[i], so, s[i]);
-                a[i] *= ao;
-            }
-        }
-    }
-    const bool edge = FWD ? lane < CX : lane >= 64 - CX;        // first group in walking order
+    const int row = lane >> 4;
+    const bool odd = row & 1, upper = row & 2;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        const float ao = FWD ? __shfl_up(a[i], CX) : __shfl_down(a[i], CX);
-        const float so = FWD ? __shfl_up(s[i], CX) : __shfl_down(s[i], CX);
-        Ae[i] = (GW == 1 || edge) ? 1.f : ao;
-        Se[i] = (GW == 1 || edge) ? 0.f : so;
-    }
-    const int last = FWD ? 64 - CX + lane % CX : lane % CX;     // lane with the wave's composition
-    if constexpr (WT == 1) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) At[i] = __shfl(a[i], last), St[i] = __shfl(s[i], last);
-    } else {
-        if (lane == last) {
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                lds[((wave * CX + lane % CX) * V + i) * 2] = a[i];
-                lds[((wave * CX + lane % CX) * V + i) * 2 + 1] = s[i];
+        float a = A[i], s = S[i];
+        Ae[i] = 1.f, Se[i] = 0.f;
+        if constexpr (GW == 4) {
+            // step 1: within pairs of rows; step 2: the other pair's composition, which both its rows hand over
+            const float a1 = FWD ? lo16(a) : hi16(a), s1 = FWD ? lo16(s) : hi16(s);
+            const bool second = FWD ? odd : !odd;               // second of its pair in walking order
+            s = second ? fmaf(a, s1, s) : s;
+            a = second ? a * a1 : a;
+            const float pa = FWD ? hi16(a) : lo16(a), ps = FWD ? hi16(s) : lo16(s);                 // a pair's composition, in both its rows
+            const float a2 = FWD ? lo32(pa) : hi32(pa), s2 = FWD ? lo32(ps) : hi32(ps);             // the first pair's, everywhere
+            const bool later = FWD ? upper : !upper;
+            const float ea = second ? a1 : 1.f, es = second ? s1 : 0.f;                             // before my row, inside its pair
+            Ae[i] = later ? ea * a2 : ea;
+            Se[i] = later ? fmaf(ea, s2, es) : es;
+            if constexpr (WT == 1) {                            // all four rows: second pair after the first
+                const float a3 = FWD ? hi32(pa) : lo32(pa), s3 = FWD ? hi32(ps) : lo32(ps);
+                At[i] = a2 * a3;
+                St[i] = fmaf(a3, s2, s3);
+            } else {
+                s = later ? fmaf(a, s2, s) : s;
+                a = later ? a * a2 : a;
+            }
+        } else if constexpr (WT == 1) {
+            At[i] = a, St[i] = s;
+        }
+        if constexpr (WT > 1) {
+            if (lane / CX == (FWD ? GW - 1 : 0)) {              // last row in walking order: the wave's composition
+                lds[((wave * CX + lane % CX) * V + i) * 2] = a;
+                lds[((wave * CX + lane % CX) * V + i) * 2 + 1] = s;
             }
         }
+    }
+    if constexpr (WT > 1) {
         __syncthreads();
         float pa[V], ps[V];
 #pragma unroll
@@ -188,9 +216,80 @@ __device__ __forceinline__ void join_splits(const float* __restrict__ agg, int64
     join<V, WT, GW, FWD>(A, S, Ae, Se, At, St, p.lane, p.wave, lds);
 }
 
+// ---- splits: each one's composition (A, S), forwards or backwards --------------------------------------------------------------
+// Every thread walks a stretch of its own (split_len / 16 steps) and the workgroup joins once, so this pass is loads and three operations per element.
+// CN / HAT: how q_check / q_hat are loaded (CN: V elements or one; HAT: 0 no q_hat, 1 V elements, 2 one).
+template <typename D, int V, bool FWD, bool CN, int HAT>
+__global__ __launch_bounds__(256) void recur_split_kernel(const D* __restrict__ in, Gate gc, Gate gh, const int32_t* __restrict__ lengths,
+                                                          float* __restrict__ agg, Dims d) {
+    constexpr int WT = 4, GW = 4, kU = 8;
+    using P = Place<V, WT, GW>;
+    __shared__ float s_join[WT * P::CX * V * 2];
+    const P p(d);
+    if (!p.work) return;
+    if (p.split == (FWD ? d.splits - 1 : 0)) return;            // (uniform) nothing starts behind the last split
+    int len = d.T;
+    if (lengths) len = min(max(lengths[p.b], 0), d.T);
+    const int pc = p.on ? p.c : d.C - V;
+    const int64_t all = (int64_t)d.B * d.C;
+    const int q = d.split_len / (WT * GW), lo = p.split * d.split_len + p.tg * q, hi = min(lo + q, len);
+    const int64_t C = d.C;
+    const D* pi = in ? in + ((int64_t)p.b * d.T + lo) * C + pc : nullptr;
+    const D* pg = static_cast<const D*>(gc.p) + p.b * gc.sb + (int64_t)lo * gc.st + gate_coff(gc, pc, d.N);
+    const D* ph = HAT ? static_cast<const D*>(gh.p) + p.b * gh.sb + (int64_t)lo * gh.st + gate_coff(gh, pc, d.N) : nullptr;
+    float A[V], S[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) A[i] = 1.f, S[i] = 0.f;
+    auto take = [&](const gf_vec<D, V>& ra, const gf_vec<D, V>& rb, const gf_vec<D, V>& rq) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const float a = pick<D, V, CN>(ra, i);
+            float b = gf_to_f<D>(rb.e[i]);
+            if (HAT) b *= pick<D, V, HAT == 1>(rq, i);
+            S[i] = FWD ? fmaf(a, S[i], b) : a * (b + S[i]);
+            A[i] *= a;
+        }
+    };
+    const int n = max(hi - lo, 0), whole = in ? n / kU * kU : 0;
+    // forwards: eight steps at a time, then the rest; backwards: the rest first
+    auto eight = [&](int k) {
+        gf_vec<D, V> ra[kU], rb[kU], rq[kU];
+#pragma unroll
+        for (int l = 0; l < kU; ++l) {
+            load_one<D, V, true>(reinterpret_cast<const char*>(pi + (k + l) * C), rb[l]);
+            load_one<D, V, CN>(reinterpret_cast<const char*>(pg + (int64_t)(k + l) * gc.st), ra[l]);
+            if (HAT) load_one<D, V, HAT == 1>(reinterpret_cast<const char*>(ph + (int64_t)(k + l) * gh.st), rq[l]);
+        }
+#pragma unroll
+        for (int e = 0; e < kU; ++e) take(ra[FWD ? e : kU - 1 - e], rb[FWD ? e : kU - 1 - e], rq[FWD ? e : kU - 1 - e]);
+    };
+    auto one = [&](int k) {
+        gf_vec<D, V> ra, rb, rq;
+#pragma unroll
+        for (int i = 0; i < V; ++i) rb.e[i] = gf_from_f<D>(0.f);
+        if (in) load_one<D, V, true>(reinterpret_cast<const char*>(pi + k * C), rb);
+        load_one<D, V, CN>(reinterpret_cast<const char*>(pg + (int64_t)k * gc.st), ra);
+        if (HAT) load_one<D, V, HAT == 1>(reinterpret_cast<const char*>(ph + (int64_t)k * gh.st), rq);
+        take(ra, rb, rq);
+    };
+    if (FWD) {
+        for (int k = 0; k < whole; k += kU) eight(k);
+        for (int k = whole; k < n; ++k) one(k);
+    } else {
+        for (int k = n - 1; k >= whole; --k) one(k);
+        for (int k = whole - kU; k >= 0; k -= kU) eight(k);
+    }
+    float Ae[V], Se[V], At[V], St[V];
+    join<V, WT, GW, FWD>(A, S, Ae, Se, At, St, p.lane, p.wave, s_join);
+    if (p.on && p.tg == 0) {
+        float* g = agg + 2 * (int64_t)p.split * all + (int64_t)p.b * d.C + pc;
+#pragma unroll
+        for (int i = 0; i < V; ++i) g[i] = At[i], g[all + i] = St[i];
+    }
+}
+
 // ---- forward -------------------------------------------------------------------------------------------------------------
-// AGG: the first kernel of a split run -- no outputs but each split's (A, h)
-template <typename D, int V, int WT, int GW, bool AGG>
+template <typename D, int V, int WT, int GW, bool CN, int HAT>
 __global__ __launch_bounds__(64 * (WT == 1 ? 4 : WT)) void recur_fwd_kernel(const D* __restrict__ u, Gate gc, Gate gh, const float* __restrict__ z0,
                                                                             const int32_t* __restrict__ lengths, D* __restrict__ z,
                                                                             float* __restrict__ zT, float* __restrict__ ckpt,
@@ -198,22 +297,23 @@ __global__ __launch_bounds__(64 * (WT == 1 ? 4 : WT)) void recur_fwd_kernel(cons
     using P = Place<V, WT, GW>;
     __shared__ float s_join[WT == 1 ? 1 : 2][WT == 1 ? 1 : WT * P::CX * V * 2];
     const P p(d);
-    if (AGG && p.split == d.splits - 1) return;                 // nothing starts behind the last split
+    if (!p.work) return;
     int len = d.T;
     if (lengths) len = min(max(lengths[p.b], 0), d.T);
     const int pc = p.on ? p.c : d.C - V;                        // lanes behind the last channel read its values and store nothing
-    const int64_t ub = (int64_t)p.b * d.T * d.C + pc, chan = (int64_t)p.b * d.C + pc, all = (int64_t)d.B * d.C;
-    const int64_t cb = p.b * gc.sb + gate_coff(gc, pc, d.N), hb = p.b * gh.sb + gate_coff(gh, pc, d.N);
-    float carry[V], Asum[V];
+    const int64_t chan = (int64_t)p.b * d.C + pc, all = (int64_t)d.B * d.C;
+    const int wrow = WT == 1 ? 0 : p.wave * GW * kL, lrow = p.lane / P::CX * kL;
+    const Stream su = stream<D>(u, (int64_t)p.b * d.T * d.C, wrow, lrow, d.C, pc), sz = stream<D>(z, (int64_t)p.b * d.T * d.C, wrow, lrow, d.C, pc);
+    const Stream sc = stream<D>(gc.p, p.b * gc.sb, wrow, lrow, gc.st, gate_coff(gc, pc, d.N));
+    const Stream sh = stream<D>(gh.p, p.b * gh.sb, wrow, lrow, gh.st, gate_coff(gh, pc, d.N));
+    float carry[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) carry[i] = 0.f, Asum[i] = 1.f;
-    if (!AGG) {
-        if (z0) {
+    for (int i = 0; i < V; ++i) carry[i] = 0.f;
+    if (z0) {
 #pragma unroll
-            for (int i = 0; i < V; ++i) carry[i] = z0[chan + i];
-        }
+        for (int i = 0; i < V; ++i) carry[i] = z0[chan + i];
     }
-    if (!AGG && p.split > 0) {                                  // (uniform) the splits before this one
+    if (p.split > 0) {                                  // (uniform) the splits before this one
         float At[V], St[V];
         join_splits<V, WT, GW, true>(agg, all, chan, 0, p.split, p, At, St, s_join[WT == 1 ? 0 : 1]);
 #pragma unroll
@@ -223,38 +323,32 @@ __global__ __launch_bounds__(64 * (WT == 1 ? 4 : WT)) void recur_fwd_kernel(cons
     const int live_end = min(tend, len);
     gf_vec<D, V> ra[kL], rb[kL], rq[kL];
     auto fetch = [&](int ts) {
-        int t[kL];
-#pragma unroll
-        for (int l = 0; l < kL; ++l) t[l] = min(ts + p.tg * kL + l, len - 1);
-        load_rows<D, V>(u + ub, d.C, t, rb);
-        load_gate<D, V>(gc, cb, t, ra);
-        if (gh.p) load_gate<D, V>(gh, hb, t, rq);
+        const bool inside = ts + P::SLAB <= d.T;                // (uniform)
+        load_slab<D, V, true>(su, ts, inside, len - 1, rb);
+        load_slab<D, V, CN>(sc, ts, inside, len - 1, ra);
+        if (HAT) load_slab<D, V, HAT == 1>(sh, ts, inside, len - 1, rq);
     };
     if (tbeg < live_end) fetch(tbeg);
     int flip = 0;
     for (int ts = tbeg; ts < tend; ts += P::SLAB, flip ^= 1) {
         const int t0 = ts + p.tg * kL;
         if (ts >= len) {                                        // (uniform) behind the sequence: the state stays, the output is zero
-            if (!AGG && p.on) {
+            if (p.on) {
                 const float zero[V] = {};
                 for (int l = 0; l < kL; ++l)
-                    if (t0 + l < d.T) gf_store<D, V>(z + ub + (int64_t)(t0 + l) * d.C, zero);
+                    if (t0 + l < d.T) gf_store<D, V>(reinterpret_cast<D*>(sz.at(ts + l)), zero);
             }
             continue;
         }
         float a[kL][V], b[kL][V], A[V], S[V];
-        spread_gate<D, V>(gc, ra);
 #pragma unroll
         for (int l = 0; l < kL; ++l)
 #pragma unroll
-            for (int i = 0; i < V; ++i) a[l][i] = gf_to_f<D>(ra[l].e[i]), b[l][i] = gf_to_f<D>(rb[l].e[i]);
-        if (gh.p) {
-            spread_gate<D, V>(gh, rq);
-#pragma unroll
-            for (int l = 0; l < kL; ++l)
-#pragma unroll
-                for (int i = 0; i < V; ++i) b[l][i] *= gf_to_f<D>(rq[l].e[i]);
-        }
+            for (int i = 0; i < V; ++i) {
+                a[l][i] = pick<D, V, CN>(ra[l], i);
+                b[l][i] = gf_to_f<D>(rb[l].e[i]);
+                if (HAT) b[l][i] *= pick<D, V, HAT == 1>(rq[l], i);
+            }
         if (ts + P::SLAB < live_end) fetch(ts + P::SLAB);       // (into the registers just read: the next slab loads while this one is joined)
         if (ts + P::SLAB > len) {                               // (uniform) the sequence ends in this slab
 #pragma unroll
@@ -278,36 +372,38 @@ __global__ __launch_bounds__(64 * (WT == 1 ? 4 : WT)) void recur_fwd_kernel(cons
         for (int i = 0; i < V; ++i) {
             h[i] = fmaf(Ae[i], carry[i], Se[i]);
             carry[i] = fmaf(At[i], carry[i], St[i]);
-            Asum[i] *= At[i];
         }
-        if (!AGG && p.on) {
+        if (p.on) {
             if (ckpt && t0 < d.T && t0 % d.every == 0) {
                 float* k = ckpt + ((int64_t)p.b * d.nck + t0 / d.every) * d.C + pc;
 #pragma unroll
                 for (int i = 0; i < V; ++i) k[i] = h[i];
             }
+            if (ts + P::SLAB <= len) {
 #pragma unroll
-            for (int l = 0; l < kL; ++l) {
-                if (t0 + l < d.T) {
-                    float o[V];
+                for (int l = 0; l < kL; ++l) {
 #pragma unroll
-                    for (int i = 0; i < V; ++i) {
-                        h[i] = fmaf(a[l][i], h[i], b[l][i]);
-                        o[i] = t0 + l < len ? h[i] : 0.f;
+                    for (int i = 0; i < V; ++i) h[i] = fmaf(a[l][i], h[i], b[l][i]);
+                    gf_store<D, V>(reinterpret_cast<D*>(sz.at(ts + l)), h);
+                }
+            } else {
+#pragma unroll
+                for (int l = 0; l < kL; ++l) {
+                    if (t0 + l < d.T) {
+                        float o[V];
+#pragma unroll
+                        for (int i = 0; i < V; ++i) {
+                            h[i] = fmaf(a[l][i], h[i], b[l][i]);
+                            o[i] = t0 + l < len ? h[i] : 0.f;
+                        }
+                        gf_store<D, V>(reinterpret_cast<D*>(sz.at(ts + l)), o);
                     }
-                    gf_store<D, V>(z + ub + (int64_t)(t0 + l) * d.C, o);
                 }
             }
         }
     }
     if (p.on && p.tg == 0) {
-        if (AGG) {
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                agg[(2 * (int64_t)p.split) * all + chan + i] = Asum[i];
-                agg[(2 * (int64_t)p.split + 1) * all + chan + i] = carry[i];
-            }
-        } else if (p.split == d.splits - 1) {
+        if (p.split == d.splits - 1) {
 #pragma unroll
             for (int i = 0; i < V; ++i) zT[chan + i] = carry[i];
         }
@@ -322,23 +418,33 @@ struct GateOut {
     int32_t mode;
 };
 
+template <int CTRL> __device__ __forceinline__ float row_shift(float v) {       // the lane that many below in the row, 0 at its start
+    return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), CTRL, 0xf, 0xf, false));
+}
+
 template <typename D, int V, int CX>
-__device__ __forceinline__ void put_gate(const GateOut& g, const float (&v)[V], int64_t off, int64_t toff, bool on, bool live, int lane) {
+__device__ __forceinline__ void put_gate(const GateOut& g, const float (&v)[V], char* direct, int64_t off, int64_t toff, bool on, bool live, int lane) {
     if (g.mode == kOutDirect) {
-        if (on && live) gf_store<D, V>(static_cast<D*>(g.p) + off, v);
+        if (on && live) gf_store<D, V>(reinterpret_cast<D*>(direct), v);
     } else if (g.mode == kOutProduct) {
         if (on && live) gf_store<float, V>(static_cast<float*>(g.p) + off, v);
     } else if (g.mode == kOutTime) {
         float s = 0.f;
 #pragma unroll
         for (int i = 0; i < V; ++i) s += on ? v[i] : 0.f;
-#pragma unroll
-        for (int off2 = 1; off2 < CX; off2 <<= 1) s += __shfl_xor(s, off2);
-        if (live && lane % CX == 0) static_cast<float*>(g.p)[toff] = s;
+        s += row_shift<0x111>(s);                               // over the row of 16 lanes: its last lane has the sum
+        s += row_shift<0x112>(s);
+        s += row_shift<0x114>(s);
+        s += row_shift<0x118>(s);
+        if constexpr (CX == 64) {
+            s += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(s), 0x142, 0xa, 0xf, false));
+            s += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(s), 0x143, 0xc, 0xf, false));
+        }
+        if (live && lane % CX == CX - 1) static_cast<float*>(g.p)[toff] = s;
     }
 }
 
-template <typename D, int V, int WT, int GW, bool AGG>
+template <typename D, int V, int WT, int GW, bool CN, int HAT>
 __global__ __launch_bounds__(64 * (WT == 1 ? 4 : WT)) void recur_bwd_kernel(const D* __restrict__ u, Gate gc, Gate gh, const int32_t* __restrict__ lengths,
                                                                             const D* __restrict__ dz, const float* __restrict__ dzT,
                                                                             const float* __restrict__ ckpt, D* __restrict__ du, GateOut oc, GateOut oh,
@@ -346,25 +452,28 @@ __global__ __launch_bounds__(64 * (WT == 1 ? 4 : WT)) void recur_bwd_kernel(cons
     using P = Place<V, WT, GW>;
     __shared__ float s_join[WT == 1 ? 1 : 4][WT == 1 ? 1 : WT * P::CX * V * 2];
     const P p(d);
-    if (AGG && p.split == 0) return;
+    if (!p.work) return;
     int len = d.T;
     if (lengths) len = min(max(lengths[p.b], 0), d.T);
     const int pc = p.on ? p.c : d.C - V;
     const int64_t ub = (int64_t)p.b * d.T * d.C + pc, chan = (int64_t)p.b * d.C + pc, all = (int64_t)d.B * d.C;
-    const int64_t cb = p.b * gc.sb + gate_coff(gc, pc, d.N), hb = p.b * gh.sb + gate_coff(gh, pc, d.N);
+    const int wrow = WT == 1 ? 0 : p.wave * GW * kL, lrow = p.lane / P::CX * kL;
+    const int64_t first = (int64_t)p.b * d.T * d.C;
+    const Stream su = stream<D>(u, first, wrow, lrow, d.C, pc), sg = stream<D>(dz, first, wrow, lrow, d.C, pc), so = stream<D>(du, first, wrow, lrow, d.C, pc);
+    const Stream soc = stream<D>(oc.p, first, wrow, lrow, d.C, pc), soh = stream<D>(oh.p, first, wrow, lrow, d.C, pc);
+    const Stream sc = stream<D>(gc.p, p.b * gc.sb, wrow, lrow, gc.st, gate_coff(gc, pc, d.N));
+    const Stream sh = stream<D>(gh.p, p.b * gh.sb, wrow, lrow, gh.st, gate_coff(gh, pc, d.N));
     // sums over a wave's channels (time gates): one row of [B, T] per wave column
-    const int64_t cols = (int64_t)(blockIdx.x % (unsigned)d.chunks) * (WT == 1 ? P::NW : 1) + (WT == 1 ? p.wave : 0);
+    const int64_t cols = (int64_t)p.column * (WT == 1 ? P::NW : 1) + (WT == 1 ? p.wave : 0);
     const int64_t tbase = (cols * d.B + p.b) * d.T;
-    float carry[V], Asum[V];
+    float carry[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) carry[i] = 0.f, Asum[i] = 1.f;
-    if (!AGG) {
-        if (dzT) {
+    for (int i = 0; i < V; ++i) carry[i] = 0.f;
+    if (dzT) {
 #pragma unroll
-            for (int i = 0; i < V; ++i) carry[i] = dzT[chan + i];
-        }
+        for (int i = 0; i < V; ++i) carry[i] = dzT[chan + i];
     }
-    if (!AGG && p.split + 1 < d.splits) {                       // (uniform) the splits behind this one
+    if (p.split + 1 < d.splits) {                       // (uniform) the splits behind this one
         float At[V], St[V];
         join_splits<V, WT, GW, false>(agg, all, chan, p.split + 1, d.splits, p, At, St, s_join[WT == 1 ? 0 : 2]);
 #pragma unroll
@@ -374,57 +483,38 @@ __global__ __launch_bounds__(64 * (WT == 1 ? 4 : WT)) void recur_bwd_kernel(cons
     const int slabs = tend > tbeg ? (tend - tbeg + P::SLAB - 1) / P::SLAB : 0;
     gf_vec<D, V> ra[kL], rx[kL], rq[kL], rg[kL];
     auto fetch = [&](int ts) {
-        int t[kL];
-#pragma unroll
-        for (int l = 0; l < kL; ++l) t[l] = min(ts + p.tg * kL + l, len - 1);
-        if (dz) load_rows<D, V>(dz + ub, d.C, t, rg);
-        load_gate<D, V>(gc, cb, t, ra);
-        if (!AGG) {
-            load_rows<D, V>(u + ub, d.C, t, rx);
-            if (gh.p) load_gate<D, V>(gh, hb, t, rq);
-        }
+        const bool inside = ts + P::SLAB <= d.T;                // (uniform)
+        if (dz) load_slab<D, V, true>(sg, ts, inside, len - 1, rg);
+        load_slab<D, V, true>(su, ts, inside, len - 1, rx);
+        load_slab<D, V, CN>(sc, ts, inside, len - 1, ra);
+        if (HAT) load_slab<D, V, HAT == 1>(sh, ts, inside, len - 1, rq);
     };
     if (tbeg < min(tend, len)) fetch(tbeg + (min(tend, len) - tbeg - 1) / P::SLAB * P::SLAB);     // the last slab with a live step
     int flip = 0;
     for (int sl = slabs - 1; sl >= 0; --sl, flip ^= 2) {
         const int ts = tbeg + sl * P::SLAB, t0 = ts + p.tg * kL;
         if (ts >= len) {                                        // (uniform) behind the sequence: nothing flows, the gradients are zero
-            if (!AGG) {
-                const float zero[V] = {};
-                for (int l = 0; l < kL; ++l) {
-                    const int64_t off = ub + (int64_t)(t0 + l) * d.C;
-                    if (du && p.on && t0 + l < d.T) gf_store<D, V>(du + off, zero);
-                    if (oc.mode) put_gate<D, V, P::CX>(oc, zero, off, tbase + t0 + l, p.on, t0 + l < d.T, p.lane);
-                    if (oh.mode) put_gate<D, V, P::CX>(oh, zero, off, tbase + t0 + l, p.on, t0 + l < d.T, p.lane);
-                }
+            const float zero[V] = {};
+            for (int l = 0; l < kL; ++l) {
+                const int64_t off = ub + (int64_t)(t0 + l) * d.C;
+                const bool in = t0 + l < d.T;
+                if (du && p.on && in) gf_store<D, V>(reinterpret_cast<D*>(so.at(ts + l)), zero);
+                if (oc.mode) put_gate<D, V, P::CX>(oc, zero, soc.at(ts + l), off, tbase + t0 + l, p.on, in, p.lane);
+                if (HAT && oh.mode) put_gate<D, V, P::CX>(oh, zero, soh.at(ts + l), off, tbase + t0 + l, p.on, in, p.lane);
             }
             continue;
         }
         const bool ends = ts + P::SLAB > len;                   // (uniform) the sequence ends in this slab
         float a[kL][V], x[kL][V], q[kL][V], g[kL][V], A[V], R[V];
-        spread_gate<D, V>(gc, ra);
 #pragma unroll
         for (int l = 0; l < kL; ++l)
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                a[l][i] = gf_to_f<D>(ra[l].e[i]);
-                g[l][i] = 0.f;
-                x[l][i] = AGG ? 0.f : gf_to_f<D>(rx[l].e[i]);
-                q[l][i] = 1.f;
+                a[l][i] = pick<D, V, CN>(ra[l], i);
+                x[l][i] = gf_to_f<D>(rx[l].e[i]);
+                q[l][i] = HAT ? pick<D, V, HAT == 1>(rq[l], i) : 1.f;
+                g[l][i] = dz ? gf_to_f<D>(rg[l].e[i]) : 0.f;
             }
-        if (dz) {
-#pragma unroll
-            for (int l = 0; l < kL; ++l)
-#pragma unroll
-                for (int i = 0; i < V; ++i) g[l][i] = gf_to_f<D>(rg[l].e[i]);
-        }
-        if (!AGG && gh.p) {
-            spread_gate<D, V>(gh, rq);
-#pragma unroll
-            for (int l = 0; l < kL; ++l)
-#pragma unroll
-                for (int i = 0; i < V; ++i) q[l][i] = gf_to_f<D>(rq[l].e[i]);
-        }
         if (sl > 0) fetch(ts - P::SLAB);                        // (into the registers just read: the next slab loads while this one is joined)
         if (ends) {
 #pragma unroll
@@ -448,9 +538,8 @@ __global__ __launch_bounds__(64 * (WT == 1 ? 4 : WT)) void recur_bwd_kernel(cons
         for (int i = 0; i < V; ++i) {
             r[i] = fmaf(Ae[i], carry[i], Re[i]);
             carry[i] = fmaf(At[i], carry[i], Rt[i]);
-            Asum[i] *= At[i];
         }
-        if (!AGG) {
+        {
             float zp[kL][V];
             if (oc.mode != kOutNone) {                          // the states z_{t-1} of this slab, from its checkpoint
                 float S[V], h[V], Se[V], St[V];
@@ -459,7 +548,7 @@ __global__ __launch_bounds__(64 * (WT == 1 ? 4 : WT)) void recur_bwd_kernel(cons
 #pragma unroll
                 for (int l = 0; l < kL; ++l)
 #pragma unroll
-                    for (int i = 0; i < V; ++i) S[i] = fmaf(a[l][i], S[i], x[l][i] * q[l][i]);
+                    for (int i = 0; i < V; ++i) S[i] = fmaf(a[l][i], S[i], HAT ? x[l][i] * q[l][i] : x[l][i]);
                 join<V, WT, GW, true>(A, S, Ae, Se, At, St, p.lane, p.wave, s_join[WT == 1 ? 0 : flip + 1]);
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
@@ -471,7 +560,7 @@ __global__ __launch_bounds__(64 * (WT == 1 ? 4 : WT)) void recur_bwd_kernel(cons
 #pragma unroll
                     for (int i = 0; i < V; ++i) {
                         zp[l][i] = h[i];
-                        h[i] = fmaf(a[l][i], h[i], x[l][i] * q[l][i]);
+                        h[i] = fmaf(a[l][i], h[i], HAT ? x[l][i] * q[l][i] : x[l][i]);
                     }
             }
 #pragma unroll
@@ -482,7 +571,7 @@ __global__ __launch_bounds__(64 * (WT == 1 ? 4 : WT)) void recur_bwd_kernel(cons
                     const float gt = g[l][i] + r[i];            // dL/dz_t
                     o[i] = gt * zp[l][i];
                     oq[i] = gt * x[l][i];
-                    ox[i] = gt * q[l][i];
+                    ox[i] = HAT ? gt * q[l][i] : gt;
                     r[i] = a[l][i] * gt;
                 }
                 bool in = true;
@@ -493,20 +582,14 @@ __global__ __launch_bounds__(64 * (WT == 1 ? 4 : WT)) void recur_bwd_kernel(cons
                         if (t0 + l >= len) o[i] = oq[i] = ox[i] = 0.f;
                 }
                 const int64_t off = ub + (int64_t)(t0 + l) * d.C;
-                if (du && p.on && in) gf_store<D, V>(du + off, ox);
-                if (oc.mode) put_gate<D, V, P::CX>(oc, o, off, tbase + t0 + l, p.on, in, p.lane);
-                if (oh.mode) put_gate<D, V, P::CX>(oh, oq, off, tbase + t0 + l, p.on, in, p.lane);
+                if (du && p.on && in) gf_store<D, V>(reinterpret_cast<D*>(so.at(ts + l)), ox);
+                if (oc.mode) put_gate<D, V, P::CX>(oc, o, soc.at(ts + l), off, tbase + t0 + l, p.on, in, p.lane);
+                if (HAT && oh.mode) put_gate<D, V, P::CX>(oh, oq, soh.at(ts + l), off, tbase + t0 + l, p.on, in, p.lane);
             }
         }
     }
     if (p.on && p.tg == 0) {
-        if (AGG) {
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                agg[(2 * (int64_t)p.split) * all + chan + i] = Asum[i];
-                agg[(2 * (int64_t)p.split + 1) * all + chan + i] = carry[i];
-            }
-        } else if (p.split == 0 && dz0) {
+        if (p.split == 0 && dz0) {
 #pragma unroll
             for (int i = 0; i < V; ++i) dz0[chan + i] = carry[i];
         }
@@ -585,7 +668,7 @@ Shape choose(int B, int T, int64_t C, int N, int kinds) {
     const int64_t blocks = (int64_t)B * ((C + (int64_t)(s.WT == 1 ? 4 : 1) * (64 / s.GW) * s.V - 1) / ((int64_t)(s.WT == 1 ? 4 : 1) * (64 / s.GW) * s.V));
     const int slabs = (T + s.slab - 1) / s.slab;
     s.splits = 1;
-    if (blocks < 256 && slabs >= 8) {                           // fewer workgroups than compute units and a long way to walk
+    if (s.WT == 4 && blocks < 256 && slabs >= 8) {                           // fewer workgroups than compute units and a long way to walk
         int64_t want = (2048 + blocks - 1) / blocks;
         if (want > slabs / 4) want = slabs / 4;
         if (want > kMaxSplit) want = kMaxSplit;
@@ -621,7 +704,7 @@ int check_dims(const char* who, int B, int T, int H, int N, int dtype, int kc, i
     GF_REQUIRE_ARG(gf_dtype_ok(dtype), "%s: dtype %d", who, dtype);
     GF_REQUIRE_ARG((kc & ~7) == 0 && (kh & ~7) == 0, "%s: gate kinds %d, %d", who, kc, kh);
     GF_REQUIRE_SHAPE(B > 0 && T >= 0 && H > 0 && N > 0, "%s: bad shape B=%d T=%d H=%d N=%d", who, B, T, H, N);
-    GF_REQUIRE_SHAPE((int64_t)H * N < (1ll << 30), "%s: H * N = %lld channels", who, (long long)H * N);
+    GF_REQUIRE_SHAPE((int64_t)H * N < (1ll << 26), "%s: H * N = %lld channels", who, (long long)H * N);   // (a lane's byte offset is 32 bits: 13 rows)
     GF_REQUIRE_SHAPE(T <= INT32_MAX - (1 << 16), "%s: T = %d steps", who, T);                 // (a slab's end stays an int32)
     return GF_OK;
 }
@@ -637,16 +720,34 @@ Dims make_dims(const Shape& s, int B, int T, int H, int N) {
     return d;
 }
 
-template <int V, typename F>
-int by_time(const Shape& s, F&& f) {
+template <int V, int WT, int GW, typename F>
+int by_gates(bool cn, int hat, F&& f) {
+    using std::bool_constant;
     using std::integral_constant;
-    if (s.GW == 1) return f(integral_constant<int, V>(), integral_constant<int, 1>(), integral_constant<int, 1>());
-    if (s.WT == 1) return f(integral_constant<int, V>(), integral_constant<int, 1>(), integral_constant<int, kGW>());
-    return f(integral_constant<int, V>(), integral_constant<int, 4>(), integral_constant<int, kGW>());
+    const integral_constant<int, V> v;
+    const integral_constant<int, WT> wt;
+    const integral_constant<int, GW> gw;
+    if constexpr (V == 1) {                                     // one element per thread either way
+        return hat ? f(v, wt, gw, bool_constant<true>(), integral_constant<int, 1>()) : f(v, wt, gw, bool_constant<true>(), integral_constant<int, 0>());
+    } else if (cn) {
+        return hat == 0 ? f(v, wt, gw, bool_constant<true>(), integral_constant<int, 0>())
+             : hat == 1 ? f(v, wt, gw, bool_constant<true>(), integral_constant<int, 1>()) : f(v, wt, gw, bool_constant<true>(), integral_constant<int, 2>());
+    } else {
+        return hat == 0 ? f(v, wt, gw, bool_constant<false>(), integral_constant<int, 0>())
+             : hat == 1 ? f(v, wt, gw, bool_constant<false>(), integral_constant<int, 1>()) : f(v, wt, gw, bool_constant<false>(), integral_constant<int, 2>());
+    }
 }
+template <int V, typename F>
+int by_time(const Shape& s, bool cn, int hat, F&& f) {
+    if (s.GW == 1) return by_gates<V, 1, 1>(cn, hat, f);
+    return s.WT == 1 ? by_gates<V, 1, kGW>(cn, hat, f) : by_gates<V, 4, kGW>(cn, hat, f);
+}
+// f(V, WT, GW, CN, HAT) as compile-time constants
 template <typename F>
-int by_shape(const Shape& s, F&& f) {
-    return s.V == 4 ? by_time<4>(s, f) : s.V == 2 ? by_time<2>(s, f) : by_time<1>(s, f);
+int by_shape(const Shape& s, const Gate& gc, const Gate& gh, F&& f) {
+    const bool cn = gc.kind & GF_GATE_N;
+    const int hat = !gh.p ? 0 : (gh.kind & GF_GATE_N) ? 1 : 2;
+    return s.V == 4 ? by_time<4>(s, cn, hat, f) : s.V == 2 ? by_time<2>(s, cn, hat, f) : by_time<1>(s, cn, hat, f);
 }
 
 int wave_columns(const Dims& d, const Shape& s) { return d.chunks * (s.WT == 1 ? 4 : 1); }
@@ -666,16 +767,17 @@ size_t agg_floats(const Dims& d) { return d.splits > 1 ? ((size_t)2 * d.splits *
 template <typename D>
 int forward_t(const Shape& s, const Dims& d, const void* u, Gate gc, Gate gh, const float* z0, const int32_t* lengths, void* z, float* zT, float* ckpt,
               float* agg, hipStream_t st) {
-    return by_shape(s, [&](auto v, auto wt, auto gw) -> int {
-        constexpr int V = decltype(v)::value, WT = decltype(wt)::value, GW = decltype(gw)::value;
-        const dim3 grid((unsigned)((int64_t)d.chunks * d.splits * d.B)), block(64 * (WT == 1 ? 4 : WT));
+    return by_shape(s, gc, gh, [&](auto v, auto wt, auto gw, auto cn, auto hat) -> int {
+        constexpr int V = decltype(v)::value, WT = decltype(wt)::value, GW = decltype(gw)::value, HAT = decltype(hat)::value;
+        constexpr bool CN = decltype(cn)::value;
+        const dim3 grid((unsigned)((int64_t)d.chunks * (d.splits > 1 ? ((int64_t)d.splits * d.B + 7) / 8 * 8 : d.B))), block(64 * (WT == 1 ? 4 : WT));
         const D* up = static_cast<const D*>(u);
         D* zp = static_cast<D*>(z);
         if (d.splits > 1) {
-            recur_fwd_kernel<D, V, WT, GW, true><<<grid, block, 0, st>>>(up, gc, gh, z0, lengths, zp, zT, nullptr, agg, d);
-            GF_LAUNCH_CHECK("recur_fwd_kernel (splits)");
+            if constexpr (WT == 4) recur_split_kernel<D, V, true, CN, HAT><<<grid, 256, 0, st>>>(up, gc, gh, lengths, agg, d);
+            GF_LAUNCH_CHECK("recur_split_kernel");
         }
-        recur_fwd_kernel<D, V, WT, GW, false><<<grid, block, 0, st>>>(up, gc, gh, z0, lengths, zp, zT, ckpt, agg, d);
+        recur_fwd_kernel<D, V, WT, GW, CN, HAT><<<grid, block, 0, st>>>(up, gc, gh, z0, lengths, zp, zT, ckpt, agg, d);
         GF_LAUNCH_CHECK("recur_fwd_kernel");
         return GF_OK;
     });
@@ -703,16 +805,17 @@ int backward_t(const Shape& s, const Dims& d, const void* u, Gate gc, Gate gh, c
     GateOut oc{nullptr, kOutNone}, oh{nullptr, kOutNone};
     if (dqc) oc.mode = out_mode(kc), oc.p = oc.mode == kOutDirect ? dqc : pc;
     if (dqh) oh.mode = out_mode(kh), oh.p = oh.mode == kOutDirect ? dqh : ph;
-    const int rc = by_shape(s, [&](auto v, auto wt, auto gw) -> int {
-        constexpr int V = decltype(v)::value, WT = decltype(wt)::value, GW = decltype(gw)::value;
-        const dim3 grid((unsigned)((int64_t)d.chunks * d.splits * d.B)), block(64 * (WT == 1 ? 4 : WT));
+    const int rc = by_shape(s, gc, gh, [&](auto v, auto wt, auto gw, auto cn, auto hat) -> int {
+        constexpr int V = decltype(v)::value, WT = decltype(wt)::value, GW = decltype(gw)::value, HAT = decltype(hat)::value;
+        constexpr bool CN = decltype(cn)::value;
+        const dim3 grid((unsigned)((int64_t)d.chunks * (d.splits > 1 ? ((int64_t)d.splits * d.B + 7) / 8 * 8 : d.B))), block(64 * (WT == 1 ? 4 : WT));
         const D *up = static_cast<const D*>(u), *dzp = static_cast<const D*>(dz);
         D* dup = static_cast<D*>(du);
         if (d.splits > 1) {
-            recur_bwd_kernel<D, V, WT, GW, true><<<grid, block, 0, st>>>(up, gc, gh, lengths, dzp, dzT, ckpt, dup, oc, oh, dz0, agg, d);
-            GF_LAUNCH_CHECK("recur_bwd_kernel (splits)");
+            if constexpr (WT == 4) recur_split_kernel<D, V, false, CN, 0><<<grid, 256, 0, st>>>(dzp, gc, gh, lengths, agg, d);
+            GF_LAUNCH_CHECK("recur_split_kernel");
         }
-        recur_bwd_kernel<D, V, WT, GW, false><<<grid, block, 0, st>>>(up, gc, gh, lengths, dzp, dzT, ckpt, dup, oc, oh, dz0, agg, d);
+        recur_bwd_kernel<D, V, WT, GW, CN, HAT><<<grid, block, 0, st>>>(up, gc, gh, lengths, dzp, dzT, ckpt, dup, oc, oh, dz0, agg, d);
         GF_LAUNCH_CHECK("recur_bwd_kernel");
         return GF_OK;
     });
