@@ -22,7 +22,8 @@ namespace {
 constexpr int kThr = 256;
 constexpr int kTopMax = 64;
 constexpr int kPackMax = 64;       // rows of up to so many outputs are packed into waves
-constexpr int kMaxNV = 4;          // 16-byte groups per thread and tile: 4 / 8 / 2 take 162 / 189 / 177 us for 4096 x 50001 bf16 with 8 alternatives
+constexpr int kMaxNV = 4;          // 16-byte groups per thread and tile.  8 (twice the registers, a 64-bit hit mask) and 2 lost when the alternatives were
+                                   // still collected element by element: 189 and 177 us against 162 us for 4096 x 50001 bf16 with 8 of them
 constexpr int kCand = 1024;        // candidates that are ranked in LDS; more (heavy ties) take the extraction loop
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -169,7 +170,8 @@ __global__ __launch_bounds__(kThr) void tile_kernel(const D* __restrict__ logits
     const Row<D> row(logits + r * row_stride, V);
     const int64_t g0 = (int64_t)tile * NV * kThr;
     float x[NV][VE];
-    if (row.first(g0 + NV * kThr) <= V) {                       // (uniform) a tile inside the row: plain loads
+    const bool full = row.first(g0 + NV * kThr) <= V;
+    if (full) {                                                 // (uniform) a tile inside the row: plain loads
         gf_vec_any<D, VE> raw[NV];
 #pragma unroll
         for (int v = 0; v < NV; ++v) raw[v] = *reinterpret_cast<const gf_vec_any<D, VE>*>(row.p + row.first(g0 + v * kThr + tid));
@@ -214,7 +216,8 @@ __global__ __launch_bounds__(kThr) void tile_kernel(const D* __restrict__ logits
     const float wm = wave_max(tm);
     if constexpr (TOP) {
         const unsigned o = ord32(tm);
-        const unsigned a = kth_of_wave(o, (top + 3) / 4), b = kth_of_wave(o, top);
+        // (a tile the row does not fill has waves without enough values: their own k-th largest then decides)
+        const unsigned a = kth_of_wave(o, (top + 3) / 4), b = full ? 0u : kth_of_wave(o, top);
         if (lane == 0) s_thr[wave] = a, s_thr[4 + wave] = b;
     }
     const float c2 = c * kLog2e, ref = wm == -INFINITY ? 0.f : wm;         // a wave with nothing in it: all exponentials are zero
@@ -274,19 +277,24 @@ __global__ __launch_bounds__(kThr) void tile_kernel(const D* __restrict__ logits
             for (int w = 1; w < 4; ++w) ua = min(ua, s_thr[w]), ub = max(ub, s_thr[4 + w]);
             const unsigned u = max(ua, ub);
             const float thr = u < 0x00800000u ? -INFINITY : unord32(u);   // (bits below the ordered -inf = negative NaNs)
+            static_assert(NV * VE <= 32, "a thread's elements are the bits of a mask");
+            unsigned hits = 0u;                                 // (the few hits are read again: no code per element for them)
             if (tm >= thr) {
 #pragma unroll
                 for (int v = 0; v < NV; ++v) {
                     if (vm[v] >= thr) {
-                        const int64_t j0 = row.first(g0 + v * kThr + tid);
 #pragma unroll
-                        for (int e = 0; e < VE; ++e) {
-                            if (x[v][e] >= thr && j0 + e < V) {
-                                const int k = atomicAdd(&s_n, 1);
-                                if (k < kCand) s_cand[k] = make_key(x[v][e], j0 + e);
-                            }
-                        }
+                        for (int e = 0; e < VE; ++e) hits |= x[v][e] >= thr ? 1u << (v * VE + e) : 0u;
                     }
+                }
+            }
+            while (hits) {
+                const int at2 = __ffs(hits) - 1;
+                hits &= hits - 1u;
+                const int64_t j = row.first(g0 + at2 / VE * kThr + tid) + at2 % VE;
+                if (j < V) {
+                    const int k = atomicAdd(&s_n, 1);
+                    if (k < kCand) s_cand[k] = make_key(gf_to_f<D>(row.p[j]), j);
                 }
             }
         }
@@ -308,13 +316,18 @@ __global__ __launch_bounds__(kThr) void tile_kernel(const D* __restrict__ logits
             u64 last = ~0ull;
             for (int k = 0; k < top; ++k) {
                 u64 best = 0ull;
-#pragma unroll
+                int nothing = 0;                                // (rare: the tile is read again rather than kept in registers for this,
+                asm volatile("" : "+v"(nothing));               //  so the address must look new to the compiler)
+                const Row<D> row2(row.p + nothing, V);
+#pragma unroll 1
                 for (int v = 0; v < NV; ++v) {
+                    float y[VE];
                     const int64_t j0 = row.first(g0 + v * kThr + tid);
+                    row2.load(g0 + v * kThr + tid, y, -INFINITY);
 #pragma unroll
                     for (int e = 0; e < VE; ++e) {
                         if (j0 + e < V) {
-                            const u64 key = make_key(x[v][e], j0 + e);
+                            const u64 key = make_key(y[e], j0 + e);
                             if (key < last && key > best) best = key;
                         }
                     }
@@ -720,7 +733,7 @@ template <typename D> int pick_nv(int64_t R, int64_t V) {
     const int64_t groups = row_groups<D>(V);
     for (int nv = kMaxNV; nv > 1; nv >>= 1) {
         const int64_t tiles = (groups + (int64_t)nv * kThr - 1) / ((int64_t)nv * kThr);
-        if (R * tiles >= 2048 && groups > (int64_t)(nv / 2) * kThr) return nv;
+        if (R * tiles >= 1024 && groups > (int64_t)(nv / 2) * kThr) return nv;
     }
     return groups > 64 * kThr ? 2 : 1;                          // few rows: small tiles, yet not so many that joining them counts
 }

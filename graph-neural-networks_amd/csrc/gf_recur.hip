@@ -102,8 +102,9 @@ struct Place {
         unsigned blk = blockIdx.x;
         if (d.splits > 1) {
             // Workgroups go to the 8 XCDs in turn.  Long runs put all chunks of a (sequence, split) on one XCD: a chunk's row segments (128 bytes,
-            // starting at any multiple of V elements) share their cache lines with its neighbours' (65537 x 808 bf16: 291 -> 269 us).  Without splits
-            // there is work enough to stream, and sequences of unlike lengths are better spread over the XCDs (32 x 257 x 53824: 1361 / 1513 us).
+            // starting at any multiple of V elements) share their cache lines with its neighbours' (65537 x 808 bf16, forward and backward: 248 ->
+            // 233 us).  Without splits there is work enough to stream, and sequences of unlike lengths are better spread over the XCDs
+            // (32 x 257 x 53824, lengths 0 .. 257: 1361 us spread, 1513 us with a sequence per XCD).
             const unsigned x = blk & 7u, k = blk >> 3;
             blk = (x + 8u * (k / (unsigned)d.chunks)) * (unsigned)d.chunks + k % (unsigned)d.chunks;
         }
