@@ -5,6 +5,8 @@ There is NO fallback: if the HIP library is missing or a call fails, the product
 from __future__ import annotations
 
 import ctypes
+import importlib.machinery
+import importlib.util
 import os
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -108,6 +110,27 @@ def lib():
             fn.restype, fn.argtypes = res, args
         _lib = handle
     return _lib
+
+
+_host = None
+HOST_PATH = os.path.join(_HERE, "_gf_torch.so")
+
+
+def host():
+    """The autograd nodes of the sequence and output operators (csrc/gf_torch.cpp), bound to the library lib() has loaded."""
+    global _host
+    if _host is None:
+        if not os.path.exists(HOST_PATH):
+            raise RuntimeError(f"{HOST_PATH} is missing: build it with `python -c 'import __graft_entry__ as g; g.build()'` (or `make -C "
+                               "graph-neural-networks_amd`). There is no fallback by design.")
+        import torch  # noqa: F401  (its symbols are the module's)
+        loader = importlib.machinery.ExtensionFileLoader("_gf_torch", HOST_PATH)
+        module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_gf_torch", loader))
+        loader.exec_module(module)
+        handle = lib()
+        module.bind({name: ctypes.cast(getattr(handle, name), ctypes.c_void_p).value for name in _SIGNATURES})
+        _host = module
+    return _host
 
 
 def check(rc: int, what: str = "") -> None:

@@ -613,9 +613,21 @@ __device__ __forceinline__ float sum_strided(const float* __restrict__ p, int n,
     return s;
 }
 
+struct Fold {                      // src [nb, B, T, Hs, Ns] -> out in the gate's shape
+    const float* src;
+    void* out;
+    int32_t nb, Hs, Ns, kind;
+    int64_t total;
+};
+
+// blockIdx.y: q_check's and q_hat's gradient in one launch
 template <typename D>
-__global__ __launch_bounds__(256) void recur_fold_kernel(const float* __restrict__ src, D* __restrict__ out, int nb, int B, int T, int Hs, int Ns,
-                                                         int kind, int64_t total) {
+__global__ __launch_bounds__(256) void recur_fold_kernel(Fold f0, Fold f1, int B, int T) {
+    const Fold f = blockIdx.y ? f1 : f0;
+    const float* __restrict__ src = f.src;
+    D* __restrict__ out = static_cast<D*>(f.out);
+    const int nb = f.nb, Hs = f.Hs, Ns = f.Ns, kind = f.kind;
+    const int64_t total = f.total;
     const bool byN = !(kind & GF_GATE_N) && Ns > 1;
     const int Ho = (kind & GF_GATE_H) ? Hs : 1, No = (kind & GF_GATE_N) ? Ns : 1, Bo = (kind & GF_GATE_B) ? B : 1;
     const int lane = threadIdx.x & 63;
@@ -784,17 +796,16 @@ int forward_t(const Shape& s, const Dims& d, const void* u, Gate gc, Gate gh, co
     });
 }
 
-template <typename D>
-int fold_t(const float* src, void* out, int kind, int mode, const Dims& d, const Shape& s, hipStream_t st) {
-    const int nb = mode == kOutTime ? wave_columns(d, s) : 1, Hs = mode == kOutTime ? 1 : d.H, Ns = mode == kOutTime ? 1 : d.N;
-    const int64_t total = (int64_t)((kind & GF_GATE_B) ? d.B : 1) * d.T * ((kind & GF_GATE_H) ? d.H : 1) * ((kind & GF_GATE_N) ? d.N : 1);
-    if (total == 0) return GF_OK;
-    const int64_t per = (!(kind & GF_GATE_N) && Ns > 1) ? 4 : 256;
-    int64_t blocks = (total + per - 1) / per;
-    if (blocks > 256 * 32) blocks = 256 * 32;
-    recur_fold_kernel<D><<<dim3((unsigned)blocks), dim3(256), 0, st>>>(src, static_cast<D*>(out), nb, d.B, d.T, Hs, Ns, kind, total);
-    GF_LAUNCH_CHECK("recur_fold_kernel");
-    return GF_OK;
+Fold make_fold(const float* src, void* out, int kind, int mode, const Dims& d, const Shape& s) {
+    Fold f;
+    f.src = src, f.out = out, f.kind = kind;
+    f.nb = mode == kOutTime ? wave_columns(d, s) : 1, f.Hs = mode == kOutTime ? 1 : d.H, f.Ns = mode == kOutTime ? 1 : d.N;
+    f.total = (int64_t)((kind & GF_GATE_B) ? d.B : 1) * d.T * ((kind & GF_GATE_H) ? d.H : 1) * ((kind & GF_GATE_N) ? d.N : 1);
+    return f;
+}
+int64_t fold_blocks(const Fold& f) {
+    const int64_t per = (!(f.kind & GF_GATE_N) && f.Ns > 1) ? 4 : 256, blocks = (f.total + per - 1) / per;
+    return blocks > 256 * 32 ? 256 * 32 : blocks;
 }
 
 template <typename D>
@@ -821,11 +832,16 @@ int backward_t(const Shape& s, const Dims& d, const void* u, Gate gc, Gate gh, c
         return GF_OK;
     });
     if (rc != GF_OK) return rc;
-    if (dqc && oc.mode != kOutDirect) {
-        const int r = fold_t<D>(pc, dqc, kc, oc.mode, d, s, st);
-        if (r != GF_OK) return r;
+    Fold f[2];
+    int n = 0;
+    if (d.T > 0 && dqc && oc.mode != kOutDirect) f[n++] = make_fold(pc, dqc, kc, oc.mode, d, s);
+    if (d.T > 0 && dqh && oh.mode != kOutDirect) f[n++] = make_fold(ph, dqh, kh, oh.mode, d, s);
+    if (n) {
+        if (n == 1) f[1] = f[0];
+        const int64_t a = fold_blocks(f[0]), b = fold_blocks(f[1]);
+        recur_fold_kernel<D><<<dim3((unsigned)(a > b ? a : b), (unsigned)n), dim3(256), 0, st>>>(f[0], f[1], d.B, d.T);
+        GF_LAUNCH_CHECK("recur_fold_kernel");
     }
-    if (dqh && oh.mode != kOutDirect) return fold_t<D>(ph, dqh, kh, oh.mode, d, s, st);
     return GF_OK;
 }
 

@@ -9,7 +9,7 @@ import torch
 import _seq_ref as ref
 import alegnn_amd
 from alegnn_amd import _lib, distill_top, linear_recurrence, token_log_probs
-from alegnn_amd.functional_seq import _gate_kind
+from alegnn_amd.functional_seq import _check_gate
 from alegnn_amd.modules.training import Trainer
 from alegnn_amd.utils import graphML as gml
 
@@ -127,10 +127,9 @@ def test_python_layer_refuses_what_is_not_on_the_gpu_and_wrong_shapes():
         token_log_probs(x, t, dim=2)
     for bad in ((2, 3, 4), (2, 2, 4, 5), (3, 3, 4, 5), (2, 3, 2, 5), (2, 3, 4, 2)):
         with pytest.raises(AssertionError, match="want"):
-            _gate_kind(torch.zeros(bad), u.shape, "q_check")
-    assert _gate_kind(torch.zeros(1, 3, 1, 5), u.shape, "q") == _lib.GF_GATE_N
-    assert _gate_kind(torch.zeros(2, 3, 4, 1), u.shape, "q") == _lib.GF_GATE_B | _lib.GF_GATE_H
-    assert _gate_kind(torch.zeros(1, 3, 1, 1), torch.Size((1, 3, 1, 1)), "q") == FULL             # axes of length one are there
+            _check_gate("linear_recurrence", torch.zeros(bad), u.shape, "q_check")
+    for good in ((1, 3, 1, 5), (2, 3, 4, 1), (1, 3, 1, 1), (2, 3, 4, 5)):
+        _check_gate("linear_recurrence", torch.zeros(good), u.shape, "q_check")
 
 
 def test_trainer_refuses_a_teacher_of_another_shape():
