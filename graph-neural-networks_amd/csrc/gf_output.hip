@@ -11,7 +11,10 @@
 // keys {ordered value, ~index}: distinct, so the order of collection does not matter and equal values come in index order.
 // Backward: one more read of the logits and one write; the few outputs that are named (token, alternatives, teacher's entries) are then
 // written over by the same workgroup.
-// Bound by HBM for fp32; for 16-bit logits the exponential (a quarter-rate instruction) and the conversions weigh about as much.
+// Bound by HBM; for 16-bit logits the exponential (a quarter-rate instruction) and the conversions weigh about as much.  Reached: forward over
+// 2048 x 100k bf16 102 us (4.0 TB/s), with entropy and 8 alternatives over 4096 x 50001 118-125 us (3.4); gradients 131-144 us (5.7-6.3 TB/s read
+// and written; a copy of 4 GiB 4.7, of 128 MiB 7.2); 2000 x 10k fp32: 16 + 26 us; 1M rows of 5: 43 us with 3 alternatives.
+// exp2_fast gives zero below 2^-126: a probability is off by less than that.
 // Sums are fp32 and in a fixed order; the K-wide part of the distillation loss is fp64 (a small difference of masses near one).
 #include "gf_num.h"
 

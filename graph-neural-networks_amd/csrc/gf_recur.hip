@@ -4,29 +4,32 @@
 // stretch of steps is one pair (A, h) with z_out = A z_in + h, and stretches compose: (A2, h2) o (A1, h1) = (A2 A1, A2 h1 + h2).
 // The channels c = h N + n are contiguous and independent; time is cut into tiles:
 //   thread     kL steps x V channels, all loads issued before the first use
-//   wave       GW groups of 64 / GW lanes; the groups hold consecutive stretches, joined by a shuffle scan
+//   wave       its rows of 16 lanes hold consecutive stretches (GW = 4), joined by row swaps, or all lanes are channels (GW = 1)
 //   workgroup  WT waves along time (joined through LDS, one barrier per slab) or 4 waves side by side along the channels (no barrier)
 //   slab       GW WT kL steps, walked in order with the state in registers
-//   split      few channels and a long T: the time axis is cut into S splits, a first kernel reads the inputs for each split's (A, h),
-//              the second one starts from the composition of the splits before its own (inputs are read twice)
+//   split      few channels and a long T: the time axis is cut into S splits, recur_split_kernel reads the inputs for each split's (A, h),
+//              the main kernel starts from the composition of the splits before its own (inputs are read twice)
 // Backward: with r_t = qc_t g_t the adjoint  g_t = dz_t + r_{t+1}  is the same recurrence run backwards with the same coefficients, and
 // needs the states z_{t-1} in fp32 for the gate's gradient: they are recomputed from the inputs (which qh's gradient reads anyway) and one
 // fp32 checkpoint per slab instead of being read back rounded.  Bound by HBM: forward reads u, qc, qh and writes z, backward reads u, qc,
 // qh, dz and writes du, dqc, dqh.
 //
 // State, products and sums are fp32; outputs are rounded once.  Steps at or behind a sequence's length leave the state as it is (A = 1,
-// h = 0), are not read, and their outputs and gradients are zero.
+// h = 0), whatever they hold (their values are replaced behind the load), and their outputs and gradients are zero.
 #include "gf_num.h"
 
 #include <type_traits>
 
 namespace {
 
-constexpr int kL = 4;              // steps per thread and slab.  8 steps need twice the registers and lose: backward of 32 x 257 x 53824 bf16 in 1.32 ms
-                                   // against 1.69 ms, of 65537 x 808 in 301 us against 416 us (both before the straight-line loads)
-constexpr int kGW = 4;             // time groups of a wave: 4 (rows of 16 lanes) against 8: 0.89 / 1.02 ms, against 2 with 8 steps: 0.89 / 0.97 ms
-constexpr int kMaxSplit = 128;     // splits of a long time axis: 128 / 64 / 256 give 307 / 344 / 323 us for 65537 x 808 bf16, forward and backward
+// Chosen by measurement (GPU time; the figures of a choice are from one build, later steps made both sides faster):
+constexpr int kL = 4;              // steps per thread and slab.  8 need twice the registers: backward of 32 x 257 x 53824 bf16 1.32 / 1.69 ms, 65537 x 808 301 / 416 us
+constexpr int kGW = 4;             // time groups of a wave: 4 against 8: 0.89 / 1.02 ms, against 2 with 8 steps each: 0.89 / 0.97 ms (the same backward)
+constexpr int kMaxSplit = 128;     // splits of a long time axis: 128 / 64 / 256: 307 / 344 / 323 us for 65537 x 808 bf16, forward and backward
 
+// What the kernels reach now: 32 x 257 x 53824 bf16 with lengths 0 .. 257: forward 0.47 ms, backward 0.90 ms = 4.9 TB/s of the rows they touch (a large
+// copy: 4.7); 65537 x 808 bf16 with a gate per step: split 21 + forward 53, split 32 + backward 118 us: the instructions per element (30 forward,
+// 50 backward in a join of 16 steps) weigh as much as the bytes there; 20 x 100 x 1600 fp32: forward 11, backward 20, gate sums 6 us.
 struct Gate {                      // a gate of shape [B|1, T, H|1, N|1]: element (b, t, h, n) at b sb + t st + channel offset
     const void* p;
     int64_t sb;

@@ -271,7 +271,7 @@ enum { GF_GATE_N = 1, GF_GATE_H = 2, GF_GATE_B = 4 };
 /* Gated linear recurrence  z_t = q_check_t z_{t-1} + q_hat_t u_t,  t = 1..T  (the recursion of GatedGRNN, graphML.py:1421-1462, with
  * an identity B(S) and sigma; gates as q_hat / q_check there).  u, z [B, T, H, N] dtype; q_check, q_hat dtype (q_hat NULL = 1);
  * z0 [B, H, N] fp32 (NULL = 0); lengths [B] int32 on the device (NULL = T; values are clamped to [0, T]): steps at or behind a sequence's
- * length are not read, leave the state as it is and give z = 0.  zT [B, H, N] fp32 is the last state.
+ * length leave the state as it is and give z = 0, whatever they hold.  zT [B, H, N] fp32 is the last state.
  * checkpoints (gf_recurrence_checkpoint_floats, NULL = not kept): one fp32 state every few steps, what the backward pass recomputes the
  * states from.  Products of q_check over a few hundred steps must stay finite in fp32.
  * Tensors are aligned to four elements.  B >= 1, T >= 0, H N < 2^26; B times the channel chunks (16 to 256 channels) < 2^24. */
