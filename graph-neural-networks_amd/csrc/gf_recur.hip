@@ -495,7 +495,7 @@ __global__ __launch_bounds__(64 * (WT == 1 ? 4 : WT)) void recur_bwd_kernel(cons
     };
     if (tbeg < min(tend, len)) fetch(tbeg + (min(tend, len) - tbeg - 1) / P::SLAB * P::SLAB);     // the last slab with a live step
     int flip = 0;
-    for (int sl = slabs - 1; sl >= 0; --sl, flip ^= 2) {
+    for (int sl = slabs - 1; sl >= 0; --sl) {
         const int ts = tbeg + sl * P::SLAB, t0 = ts + p.tg * kL;
         if (ts >= len) {                                        // (uniform) behind the sequence: nothing flows, the gradients are zero
             const float zero[V] = {};
@@ -591,6 +591,7 @@ __global__ __launch_bounds__(64 * (WT == 1 ? 4 : WT)) void recur_bwd_kernel(cons
                 if (HAT && oh.mode) put_gate<D, V, P::CX>(oh, oq, soh.at(ts + l), off, tbase + t0 + l, p.on, in, p.lane);
             }
         }
+        flip ^= 2;                                              // (per joined slab: the first one may not meet join_splits' buffer 2 again)
     }
     if (p.on && p.tg == 0) {
         if (p.split == 0 && dz0) {

@@ -97,6 +97,19 @@ def test_lengths_with_nan_in_the_padding(shape, kc, kh):
         assert (out["dq_check"][d] == 0).all() and (out["dq_hat"][d] == 0).all()
 
 
+@pytest.mark.parametrize("kc,kh", [("full", "full"), ("time", None)])
+def test_sequences_that_end_inside_a_split_of_the_time_axis(kc, kh):
+    """One workgroup per (sequence, split): the backward walk skips 0 to 3 slabs of 64 steps behind the end before it joins the first one."""
+    B, T, H, N = 12, 2048, 2, 4
+    ins = make(B, T, H, N, kc, kh, torch.float32, seed=8)
+    lengths = torch.tensor([257 + 53 * k for k in range(B)], dtype=torch.int32)
+    out = run(*ins[:4], lengths, *ins[4:])
+    check(out, ins, lengths, torch.float32)
+    for _ in range(3):
+        again = run(*ins[:4], lengths, *ins[4:])
+        assert all(np.array_equal(out[k], again[k]) for k in out)
+
+
 def test_no_steps_no_sequences_and_no_channels():
     z0 = torch.randn(2, 3, 4, device="cuda")
     for shape in ((2, 0, 3, 4), (0, 5, 3, 4), (2, 5, 0, 4), (2, 5, 3, 0)):
