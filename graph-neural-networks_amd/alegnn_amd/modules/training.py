@@ -19,7 +19,8 @@ checkpoints are written by rank 0 (model.py).
 ``teacherTop=(classes, logProbs)`` (superset option): two [nTrain, K] tensors, the K best classes of a teacher for every training sample with
 their log probabilities (evaluation.predictTop of the training split, K <= 64, an index outside the classes = padding).  A step then minimises
 (1 - distillWeight) * loss + distillWeight * mean distill_top(output, classes, logProbs) with what the K classes leave as one further outcome
-(distillWeight 0.5, distillTemperature 1.0: the temperature the log probabilities were taken at).  Validation keeps the plain loss.
+(distillWeight 0.5, distillTemperature 1.0: the temperature the log probabilities were taken at).  With as many entries as classes there is no
+further outcome: the entries' probabilities are then scaled to one.  Validation keeps the plain loss.
 
 ``hipGraph=True`` (superset option, GPU only): zero-grad + forward + loss + backward of a training step are captured once per
 batch size as a HIP graph and replayed; the samples are copied into the graph's static input buffers, the (all-reduce and)
@@ -140,8 +141,12 @@ class Trainer:
         lossValue = self.model.loss(yHat, y)
         if teacher is None:
             return lossValue
-        w = self.distillWeight
-        return (1.0 - w) * lossValue + w * distill_top(yHat, *teacher, temperature=self.distillTemperature, tail=True).mean()
+        w, tau = self.distillWeight, self.distillTemperature
+        classes, logProbs = teacher
+        tail = classes.shape[1] < yHat.shape[-1]
+        if not tail:                                                # every class is named: what rounding leaves to one belongs to none
+            logProbs = logProbs * tau
+        return (1.0 - w) * lossValue + w * distill_top(yHat, classes, logProbs, temperature=tau, tail=tail).mean()
 
     # ---- the step as a HIP graph (hipGraph=True) ---------------------------------------------------------------------
     def _graph_step(self, xTrain, yTrain, samplesType, indices, weight):

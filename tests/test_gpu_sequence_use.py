@@ -185,6 +185,28 @@ def test_a_student_learns_from_a_teachers_answers(tmp_path):
     assert abs(plain.train(data, 1, 16, printInterval=0, validationInterval=100)['lossTrain'][0] - float(ce)) < 1e-4
 
 
+@pytest.mark.parametrize("graph", [False, True])
+def test_a_student_of_all_the_classes(tmp_path, graph):
+    """predictTop asked for more classes than there are names them all: what rounding leaves of the teacher's mass is no further outcome."""
+    S = gso(30, 3).astype(np.float32)
+    data = Data(30)
+    teacher = model_of(S, 0, tmp_path, "all-teacher")
+    ans = predictTop(teacher, data, 'train', top=64, temperature=2.0)
+    assert ans['topClasses'].shape == (data.nTrain, 5)
+    np.random.seed(1)
+    student = model_of(S, 7, tmp_path, "all-student")
+    v = student.train(data, 2, 16, printInterval=0, validationInterval=100, teacherTop=(ans['topClasses'], ans['topLogProb']), distillWeight=1.0,
+                      distillTemperature=2.0, hipGraph=graph)
+    assert np.isfinite(v['lossTrain']).all() and all(torch.isfinite(q).all() for q in student.archit.parameters())
+    np.random.seed(1)                                               # the first step by hand
+    student = model_of(S, 7, tmp_path, "all-hand")
+    first = np.random.permutation(data.nTrain)[:16]
+    with torch.no_grad():
+        q = torch.log_softmax(student.archit(data.parts['train'][0][first].cuda()).double().cpu() / 2.0, 1)
+        p = torch.log_softmax(teacher.archit(data.parts['train'][0][first].cuda()).double().cpu() / 2.0, 1)
+    assert abs(v['lossTrain'][0] - float((p.exp() * (p - q)).sum(1).mean())) < 1e-4
+
+
 def test_recurrent_answers_end_to_end():
     """Recurrent net -> answers over the nodes at every step -> the student's loss on them; gradients against float64 autograd from the logits on."""
     torch.manual_seed(3)
