@@ -115,12 +115,12 @@ struct Parts {                     // per (row, tile): maximum, sums, and the ti
     u64* keys;
 };
 
-// Lower bound of the k-th largest of the wave's 64 values (as ordered unsigned): its upper 16 bits, found bit by bit -- exact for bf16, and for the
-// other types a few values more pass (half the steps of an exact search).
-__device__ __forceinline__ unsigned kth_of_wave(unsigned v, int k) {
+// Lower bound of the k-th largest of the wave's 64 values (as ordered unsigned): its bits from LOW up, found one by one.  LOW = 16: exact for bf16,
+// and for the other types a few values more pass (half the steps of the exact search, LOW = 0).
+template <int LOW = 16> __device__ __forceinline__ unsigned kth_of_wave(unsigned v, int k) {
     unsigned thr = 0;
 #pragma unroll
-    for (int b = 31; b >= 16; --b) {
+    for (int b = 31; b >= LOW; --b) {
         const unsigned c = thr | (1u << b);
         if (__popcll(__ballot(v >= c)) >= k) thr = c;
     }
@@ -152,6 +152,82 @@ __device__ __forceinline__ void answer_top(const TokenOut& o, int64_t at, u64 ke
     const float x = v == 0xfffffffeu ? NAN : unord32(v);
     o.top_tokens[at] = (unsigned)~(unsigned)key;
     o.top_logp[at] = (M == -INFINITY && ls == 0.f) ? -INFINITY : (x - M) * c - ls;
+}
+
+// A tile with more than kCand elements at or above its threshold: equal values, as rows of outputs that are ruled out (-inf) or all alike have them.  With
+// the threshold u exact (the k-th largest of the same maxima, all bits) every element above it is a candidate, and of those equal to it the first
+// ones in index order, counted by a scan over the threads per row of groups.  Returns the number of candidates in s_cand (more than kCand: does
+// not fit).  The tile is read again, so that the usual case keeps no registers for this.
+// (4096 x 50001 bf16 but for 20 outputs ruled out, 8 / 64 alternatives: 984 / 4971 us with the extraction loop below alone,
+// 531 / 550 us with this; 134 / 197 us without the mask.)
+template <typename D, int NV>
+__device__ __forceinline__ int collect_ties(const Row<D>& row, int64_t g0, float tm, bool full, int top, unsigned* s_thr, int* s_n, u64* s_cand) {
+    constexpr int VE = Row<D>::VE;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    __syncthreads();                                            // s_thr and s_n have been read
+    {
+        const unsigned o = ord32(tm), a = kth_of_wave<0>(o, (top + 3) / 4), b = full ? 0u : kth_of_wave<0>(o, top);
+        if (lane == 0) s_thr[wave] = a, s_thr[4 + wave] = b;
+        if (tid == 0) *s_n = 0;
+    }
+    __syncthreads();
+    unsigned ua = s_thr[0], ub = s_thr[4];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) ua = min(ua, s_thr[w]), ub = max(ub, s_thr[4 + w]);
+    const unsigned u = max(ua, ub);
+    int nothing = 0;                                            // (an address that looks new to the compiler: nothing is kept from the first read)
+    asm volatile("" : "+v"(nothing));
+    const Row<D> again(row.p + nothing, row.V);
+    auto each = [&](int v, auto&& f) {                          // f(e, ordered value, index) of the thread's elements of group row v
+        float y[VE];
+        const int64_t j0 = row.first(g0 + v * kThr + tid);
+        again.load(g0 + v * kThr + tid, y, -INFINITY);
+#pragma unroll
+        for (int e = 0; e < VE; ++e)
+            if (j0 + e < row.V) f(e, ord32(y[e]), j0 + e);
+    };
+#pragma unroll 1
+    for (int v = 0; v < NV; ++v)
+        each(v, [&](int, unsigned o, int64_t j) {
+            if (o > u) {
+                const int k = atomicAdd(s_n, 1);
+                if (k < kCand) s_cand[k] = ((u64)o << 32) | (unsigned)~(unsigned)j;
+            }
+        });
+    __syncthreads();
+    const int above = *s_n;
+    if (above >= top) return above;
+    int taken = 0;                                              // of the equal ones, so far
+#pragma unroll 1
+    for (int v = 0; v < NV && taken < top - above; ++v) {       // (uniform)
+        unsigned equal = 0u;
+        each(v, [&](int e, unsigned o, int64_t) { equal |= o == u ? 1u << e : 0u; });
+        int before = __popc(equal);                             // inclusive scan of the counts over the workgroup
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int below = __shfl_up(before, o);
+            if (lane >= o) before += below;
+        }
+        __syncthreads();
+        if (lane == 63) s_thr[wave] = (unsigned)before;
+        __syncthreads();
+        int all = 0;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            if (w == wave) before += all;
+            all += (int)s_thr[w];
+        }
+        int at = taken + before - __popc(equal);
+        const int64_t j0 = row.first(g0 + v * kThr + tid);
+        while (equal && at < top - above) {
+            const int e = __ffs(equal) - 1;
+            equal &= equal - 1u;
+            s_cand[above + at++] = ((u64)u << 32) | (unsigned)~(unsigned)(j0 + e);
+        }
+        taken += all;
+    }
+    __syncthreads();
+    return above + min(taken, top - above);
 }
 
 // ---- tile statistics (and best keys) -----------------------------------------------------------------------------------
@@ -304,6 +380,7 @@ __global__ __launch_bounds__(kThr) void tile_kernel(const D* __restrict__ logits
         __syncthreads();
         if (plain) {
             n = s_n;
+            if (n > kCand) n = collect_ties<D, NV>(row, g0, tm, full, top, s_thr, &s_n, s_cand);
             ranked = n <= kCand;
             if (ranked) {
                 for (int i = tid; i < n; i += kThr) {
@@ -315,7 +392,7 @@ __global__ __launch_bounds__(kThr) void tile_kernel(const D* __restrict__ logits
                     for (int i = n + tid; i < top; i += kThr) keys[i] = 0ull;
             }
         }
-        if (!ranked) {                                          // (uniform) heavy ties or NaN: extract the largest key below the last one, `top` times
+        if (!ranked) {                                          // (uniform) NaN, +inf, or too many above an exact threshold: extract the largest key below the last one, `top` times
             u64 last = ~0ull;
             for (int k = 0; k < top; ++k) {
                 u64 best = 0ull;

@@ -91,6 +91,44 @@ def test_tokens_masked_ignored_and_tied(V, dtype):
     check_tokens(x, tok, top, seed=V, grads=("top",))
 
 
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("V", [1100, 8192, 8201, 50001])
+@pytest.mark.parametrize("top", [1, 8, 64])
+def test_tokens_rows_of_equal_values(V, top, dtype):
+    """More values at or above a tile's threshold than are ranked at once: the alternatives are the first ones in index order all the same."""
+    g = torch.Generator().manual_seed(V + top)
+    x = torch.zeros((1100, V), dtype=torch.float32)
+    few = torch.randperm(V, generator=g)[:20]
+    x[1] = NINF                                                     # all but twenty ruled out (some tiles have none of them)
+    x[1, few] = torch.randn(20, generator=g)
+    x[2, few] = 1.0                                                 # twenty above the others, ties among themselves
+    x[3] = torch.finfo(DT[dtype]).min
+    x[3, few[:3]] = 2.0
+    x[4] = torch.randint(0, 2, (V,), generator=g).float()           # two values, three values
+    x[5] = torch.randint(0, 3, (V,), generator=g).float()
+    x[6, 1::2] = -0.0                                               # zeros of both signs are equal
+    x[7] = NINF
+    x[7, V - 1] = 0.5
+    x[8] = -(torch.arange(V) // 700).float()                        # steps: ties in the first tile only
+    x[9] = (torch.arange(V) // 700).float()
+    lane = torch.arange(V) % 2048 // 8                              # one wave's threads hold high values, one of them none
+    x[10] = torch.where(lane < 63, 5.0 + torch.rand(V, generator=g), -torch.rand(V, generator=g))
+    x[11] = torch.where(lane % 64 == 5, 1.0, 0.0)
+    x = x.to(DT[dtype])
+    with torch.no_grad():
+        logp, ent, tl, ti = token_log_probs(x.cuda(), torch.zeros(1100, dtype=torch.int64, device="cuda"), top=top)
+        lone = token_log_probs(x[:12].cuda(), torch.zeros(12, dtype=torch.int64, device="cuda"), top=top)[3]      # (fewer rows: other tiles)
+    y = (x[:12].float() + 0.0).cpu()
+    want = torch.sort(y, dim=1, descending=True, stable=True).indices[:, :top]
+    assert torch.equal(ti[:12].cpu(), want) and torch.equal(lone.cpu(), want)
+    assert (ti[12:].cpu() == torch.arange(top)).all()
+    lp = torch.log_softmax(y.double(), 1).gather(1, want)
+    e = (tl[:12].cpu().double() - lp).nan_to_num(0.0, posinf=0.0, neginf=0.0).abs()
+    # the answer is rounded three times (difference, scale, minus log of the sum), each by at most 2^-24 of about |lp|: 4 * 2^-24 |lp| where that
+    # exceeds the sum's own error (f16's lowest value is -65504: up to 0.0117 of rounding, whatever the kernel)
+    assert (e <= 1e-4 + 2.0 ** -22 * lp.nan_to_num(0.0, posinf=0.0, neginf=0.0).abs()).all() and torch.equal(torch.isinf(tl[:12].cpu()), torch.isinf(lp))
+
+
 @pytest.mark.parametrize("V", [5, 3000, 20011])
 def test_tokens_not_a_number_stays_in_its_row(V):
     x, g = logits_of(6, V, torch.float32, V)
