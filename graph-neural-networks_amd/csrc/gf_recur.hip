@@ -28,7 +28,7 @@ constexpr int kGW = 4;             // time groups of a wave: 4 against 8: 0.89 /
 constexpr int kMaxSplit = 128;     // splits of a long time axis: 128 / 64 / 256: 307 / 344 / 323 us for 65537 x 808 bf16, forward and backward
 
 // What the kernels reach now: 32 x 257 x 53824 bf16 with lengths 0 .. 257: forward 0.47 ms, backward 0.90 ms = 4.9 TB/s of the rows they touch (a large
-// copy: 4.7); 65537 x 808 bf16 with a gate per step: split 21 + forward 53, split 32 + backward 118 us: the instructions per element (30 forward,
+// copy: 4.7); 65537 x 808 bf16 with a gate per step: split 21 + forward 49, split 33 + backward 110 us: the instructions per element (30 forward,
 // 50 backward in a join of 16 steps) weigh as much as the bytes there; 20 x 100 x 1600 fp32: forward 11, backward 20, gate sums 6 us.
 struct Gate {                      // a gate of shape [B|1, T, H|1, N|1]: element (b, t, h, n) at b sb + t st + channel offset
     const void* p;
@@ -129,44 +129,55 @@ __device__ __forceinline__ float lo32(float x) { return __uint_as_float(__builti
 __device__ __forceinline__ float hi32(float x) { return __uint_as_float(__builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false)[1]); }
 
 // exclusive composition of the stretches before (FWD) / behind (!FWD) this thread's own, and of the whole slab.  GW = 4: the wave's rows of 16
-// lanes are the stretches (pairs first, then the halves); WT > 1: the waves' compositions through LDS.
-template <int V, int WT, int GW, bool FWD>
+// lanes are the stretches (pairs first, then the halves); WT > 1: the waves' compositions through LDS.  SAME: the thread's V channels share their gate,
+// so their products are one (lane swaps are no common subexpressions to the compiler; 65537 x 808 bf16, a gate per
+// step: forward 53 -> 49, backward 118 -> 110 us).
+template <int V, int WT, int GW, bool FWD, bool SAME>
 __device__ __forceinline__ void join(const float (&A)[V], const float (&S)[V], float (&Ae)[V], float (&Se)[V], float (&At)[V], float (&St)[V],
                                      int lane, int wave, float* lds) {
     static_assert(GW == 1 || GW == 4, "a wave's stretches are its rows of 16 lanes, or one");
     constexpr int CX = 64 / GW;
     const int row = lane >> 4;
     const bool odd = row & 1, upper = row & 2;
+    const bool second = FWD ? odd : !odd, later = FWD ? upper : !upper;     // second of its pair, of the second pair, in walking order
+    float a = 1.f, a1 = 1.f, a2 = 1.f, a3 = 1.f, ap = 1.f, ea = 1.f;        // products: channel i's, or all channels' (SAME)
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        float a = A[i], s = S[i];
+        const bool own = !SAME || i == 0;
+        float s = S[i];
+        if (own) a = ap = A[i];
         Ae[i] = 1.f, Se[i] = 0.f;
         if constexpr (GW == 4) {
             // step 1: within pairs of rows; step 2: the other pair's composition, which both its rows hand over
-            const float a1 = FWD ? lo16(a) : hi16(a), s1 = FWD ? lo16(s) : hi16(s);
-            const bool second = FWD ? odd : !odd;               // second of its pair in walking order
+            if (own) {
+                a = A[i];
+                a1 = FWD ? lo16(a) : hi16(a);
+                ap = second ? a * a1 : a;
+                const float pa = FWD ? hi16(ap) : lo16(ap);                 // a pair's composition, in both its rows
+                a2 = FWD ? lo32(pa) : hi32(pa);                             // the first pair's, everywhere
+                a3 = FWD ? hi32(pa) : lo32(pa);                             // the second pair's
+                ea = second ? a1 : 1.f;                                     // before my row, inside its pair
+            }
+            const float s1 = FWD ? lo16(s) : hi16(s);
             s = second ? fmaf(a, s1, s) : s;
-            a = second ? a * a1 : a;
-            const float pa = FWD ? hi16(a) : lo16(a), ps = FWD ? hi16(s) : lo16(s);                 // a pair's composition, in both its rows
-            const float a2 = FWD ? lo32(pa) : hi32(pa), s2 = FWD ? lo32(ps) : hi32(ps);             // the first pair's, everywhere
-            const bool later = FWD ? upper : !upper;
-            const float ea = second ? a1 : 1.f, es = second ? s1 : 0.f;                             // before my row, inside its pair
+            const float ps = FWD ? hi16(s) : lo16(s);
+            const float s2 = FWD ? lo32(ps) : hi32(ps);
+            const float es = second ? s1 : 0.f;
             Ae[i] = later ? ea * a2 : ea;
             Se[i] = later ? fmaf(ea, s2, es) : es;
             if constexpr (WT == 1) {                            // all four rows: second pair after the first
-                const float a3 = FWD ? hi32(pa) : lo32(pa), s3 = FWD ? hi32(ps) : lo32(ps);
+                const float s3 = FWD ? hi32(ps) : lo32(ps);
                 At[i] = a2 * a3;
                 St[i] = fmaf(a3, s2, s3);
             } else {
-                s = later ? fmaf(a, s2, s) : s;
-                a = later ? a * a2 : a;
+                s = later ? fmaf(ap, s2, s) : s;
             }
         } else if constexpr (WT == 1) {
             At[i] = a, St[i] = s;
         }
         if constexpr (WT > 1) {
             if (lane / CX == (FWD ? GW - 1 : 0)) {              // last row in walking order: the wave's composition
-                lds[((wave * CX + lane % CX) * V + i) * 2] = a;
+                lds[((wave * CX + lane % CX) * V + i) * 2] = later ? ap * a2 : ap;
                 lds[((wave * CX + lane % CX) * V + i) * 2 + 1] = s;
             }
         }
@@ -185,7 +196,7 @@ __device__ __forceinline__ void join(const float (&A)[V], const float (&S)[V], f
             }
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                const float wa = lds[((w * CX + lane % CX) * V + i) * 2], ws = lds[((w * CX + lane % CX) * V + i) * 2 + 1];
+                const float wa = lds[((w * CX + lane % CX) * V + (SAME ? 0 : i)) * 2], ws = lds[((w * CX + lane % CX) * V + i) * 2 + 1];
                 St[i] = fmaf(wa, St[i], ws);
                 At[i] *= wa;
             }
@@ -199,7 +210,7 @@ __device__ __forceinline__ void join(const float (&A)[V], const float (&S)[V], f
 }
 
 // composition of the splits [s0, s1) of the thread's channels, shared out over the time groups (walked forwards or backwards)
-template <int V, int WT, int GW, bool FWD>
+template <int V, int WT, int GW, bool FWD, bool SAME>
 __device__ __forceinline__ void join_splits(const float* __restrict__ agg, int64_t all, int64_t chan, int s0, int s1, const Place<V, WT, GW>& p,
                                             float (&At)[V], float (&St)[V], float* lds) {
     constexpr int TG = WT * GW;
@@ -212,12 +223,12 @@ __device__ __forceinline__ void join_splits(const float* __restrict__ agg, int64
         const float* g = agg + 2 * (int64_t)(FWD ? k : lo + hi - 1 - k) * all + chan;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            const float ak = g[i];
+            const float ak = g[SAME ? 0 : i];
             S[i] = fmaf(ak, S[i], g[all + i]);
             A[i] *= ak;
         }
     }
-    join<V, WT, GW, FWD>(A, S, Ae, Se, At, St, p.lane, p.wave, lds);
+    join<V, WT, GW, FWD, SAME>(A, S, Ae, Se, At, St, p.lane, p.wave, lds);
 }
 
 // ---- splits: each one's composition (A, S), forwards or backwards --------------------------------------------------------------
@@ -284,7 +295,7 @@ __global__ __launch_bounds__(256) void recur_split_kernel(const D* __restrict__ 
         for (int k = whole - kU; k >= 0; k -= kU) eight(k);
     }
     float Ae[V], Se[V], At[V], St[V];
-    join<V, WT, GW, FWD>(A, S, Ae, Se, At, St, p.lane, p.wave, s_join);
+    join<V, WT, GW, FWD, !CN>(A, S, Ae, Se, At, St, p.lane, p.wave, s_join);
     if (p.on && p.tg == 0) {
         float* g = agg + 2 * (int64_t)p.split * all + (int64_t)p.b * d.C + pc;
 #pragma unroll
@@ -319,7 +330,7 @@ __global__ __launch_bounds__(64 * (WT == 1 ? 4 : WT)) void recur_fwd_kernel(cons
     }
     if (p.split > 0) {                                  // (uniform) the splits before this one
         float At[V], St[V];
-        join_splits<V, WT, GW, true>(agg, all, chan, 0, p.split, p, At, St, s_join[WT == 1 ? 0 : 1]);
+        join_splits<V, WT, GW, true, !CN>(agg, all, chan, 0, p.split, p, At, St, s_join[WT == 1 ? 0 : 1]);
 #pragma unroll
         for (int i = 0; i < V; ++i) carry[i] = fmaf(At[i], carry[i], St[i]);
     }
@@ -371,7 +382,7 @@ __global__ __launch_bounds__(64 * (WT == 1 ? 4 : WT)) void recur_fwd_kernel(cons
                 A[i] *= a[l][i];
             }
         float Ae[V], Se[V], At[V], St[V], h[V];
-        join<V, WT, GW, true>(A, S, Ae, Se, At, St, p.lane, p.wave, s_join[WT == 1 ? 0 : flip]);
+        join<V, WT, GW, true, !CN>(A, S, Ae, Se, At, St, p.lane, p.wave, s_join[WT == 1 ? 0 : flip]);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             h[i] = fmaf(Ae[i], carry[i], Se[i]);
@@ -479,7 +490,7 @@ __global__ __launch_bounds__(64 * (WT == 1 ? 4 : WT)) void recur_bwd_kernel(cons
     }
     if (p.split + 1 < d.splits) {                       // (uniform) the splits behind this one
         float At[V], St[V];
-        join_splits<V, WT, GW, false>(agg, all, chan, p.split + 1, d.splits, p, At, St, s_join[WT == 1 ? 0 : 2]);
+        join_splits<V, WT, GW, false, !CN>(agg, all, chan, p.split + 1, d.splits, p, At, St, s_join[WT == 1 ? 0 : 2]);
 #pragma unroll
         for (int i = 0; i < V; ++i) carry[i] = fmaf(At[i], carry[i], St[i]);
     }
@@ -537,7 +548,7 @@ __global__ __launch_bounds__(64 * (WT == 1 ? 4 : WT)) void recur_bwd_kernel(cons
                 A[i] *= a[l][i];
             }
         float Ae[V], Re[V], At[V], Rt[V], r[V];
-        join<V, WT, GW, false>(A, R, Ae, Re, At, Rt, p.lane, p.wave, s_join[WT == 1 ? 0 : flip]);
+        join<V, WT, GW, false, !CN>(A, R, Ae, Re, At, Rt, p.lane, p.wave, s_join[WT == 1 ? 0 : flip]);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             r[i] = fmaf(Ae[i], carry[i], Re[i]);
@@ -553,7 +564,7 @@ __global__ __launch_bounds__(64 * (WT == 1 ? 4 : WT)) void recur_bwd_kernel(cons
                 for (int l = 0; l < kL; ++l)
 #pragma unroll
                     for (int i = 0; i < V; ++i) S[i] = fmaf(a[l][i], S[i], HAT ? x[l][i] * q[l][i] : x[l][i]);
-                join<V, WT, GW, true>(A, S, Ae, Se, At, St, p.lane, p.wave, s_join[WT == 1 ? 0 : flip + 1]);
+                join<V, WT, GW, true, !CN>(A, S, Ae, Se, At, St, p.lane, p.wave, s_join[WT == 1 ? 0 : flip + 1]);
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
                     const float start = ckpt[((int64_t)p.b * d.nck + ts / d.every) * d.C + pc + i];
