@@ -65,8 +65,9 @@ def linear_recurrence(u, q_check, q_hat=None, z0=None, lengths=None):
     ([B,T,1,1]), node ([B,T,1,N]), feature ([B,T,H,1]) or element; z0 [B,H,N] float32 (None = 0); lengths [B] int32 on u's device: how many
     steps of each sequence count (None = all; values are clamped to [0, T]).  What padded steps hold does not matter: they give z = 0 and no
     gradient.  Returns z [B,T,H,N] in u's dtype and the last state zT [B,H,N] in float32 -- what the next call takes as z0, so a sequence can
-    be fed in pieces down to single steps (T = 1) without losing the state's precision.  The state is float32 throughout; products of
-    q_check over a few hundred steps must stay finite (gates in [-1, 1] always do).  Differentiable (once) in u, q_check, q_hat and z0."""
+    be fed in pieces down to single steps (T = 1) without losing the state's precision.  The state is float32 throughout; the product of
+    q_check over any 64 consecutive steps must be finite (gates below 4 in magnitude always are), over longer stretches only the states have
+    to stay in range.  Differentiable (once) in u, q_check, q_hat and z0."""
     host = _lib.host()
     try:
         return host.linear_recurrence(u, q_check, q_hat, z0, lengths)

@@ -8,7 +8,8 @@
 //   workgroup  WT waves along time (joined through LDS, one barrier per slab) or 4 waves side by side along the channels (no barrier)
 //   slab       GW WT kL steps, walked in order with the state in registers
 //   split      few channels and a long T: the time axis is cut into S splits, recur_split_kernel reads the inputs for each split's (A, h),
-//              the main kernel starts from the composition of the splits before its own (inputs are read twice)
+//              the main kernel starts from the composition of the splits before its own (inputs are read twice).  There A has an exponent of its
+//              own: a product over thousands of gates may leave the range of a float32 where no state does
 // Backward: with r_t = qc_t g_t the adjoint  g_t = dz_t + r_{t+1}  is the same recurrence run backwards with the same coefficients, and
 // needs the states z_{t-1} in fp32 for the gate's gradient: they are recomputed from the inputs (which qh's gradient reads anyway) and one
 // fp32 checkpoint per slab instead of being read back rounded.  Bound by HBM: forward reads u, qc, qh and writes z, backward reads u, qc,
@@ -209,37 +210,96 @@ __device__ __forceinline__ void join(const float (&A)[V], const float (&S)[V], f
     }
 }
 
-// composition of the splits [s0, s1) of the thread's channels, shared out over the time groups (walked forwards or backwards)
+// A stretch longer than a slab: z_out = m 2^e z_in + s.  The product of its gates has an exponent of its own, so that it may leave the range of a
+// float32 where the states do not (gates above one while the state is zero, say): a stretch's s is in range whenever the step by step walk is,
+// and m 2^e only ever meets the state it is applied to.  e stays within 2^29 (a thread's stretch is at most 2^31 / 144 steps of |e| <= 150 / 8 each).
+struct Span {
+    float m;
+    int e;
+    float s;
+};
+__device__ __forceinline__ float span_apply(const Span& x, float z) { return ldexpf(x.m * z, x.e) + x.s; }
+__device__ __forceinline__ void span_norm(float& m, int& e) {
+    e += __builtin_amdgcn_frexp_expf(m);                        // (0 for 0, inf and NaN, which the mantissa keeps)
+    m = __builtin_amdgcn_frexp_mantf(m);
+}
+__device__ __forceinline__ Span span_after(const Span& x, const Span& y) {      // x behind y
+    Span r;
+    r.m = x.m * y.m, r.e = x.e + y.e, r.s = span_apply(x, y.s);
+    span_norm(r.m, r.e);
+    r.e = min(max(r.e, -(1 << 29)), 1 << 29);
+    return r;
+}
+// LDS of a workgroup's spans: [m, e, s][time group][channel of the workgroup]
+template <int V, int WT, int GW> constexpr int span_floats() { return 3 * WT * GW * (64 / GW) * V; }
+
+// The time groups' spans, joined in walking order: thread k < CX V answers channel k.  SAME: the V channels of a group share m and e.
 template <int V, int WT, int GW, bool FWD, bool SAME>
-__device__ __forceinline__ void join_splits(const float* __restrict__ agg, int64_t all, int64_t chan, int s0, int s1, const Place<V, WT, GW>& p,
-                                            float (&At)[V], float (&St)[V], float* lds) {
-    constexpr int TG = WT * GW;
-    const int q = (s1 - s0 + TG - 1) / TG, lo = min(s1, s0 + p.tg * q), hi = min(s1, lo + q);
-    float A[V], S[V], Ae[V], Se[V];
+__device__ __forceinline__ Span join_groups(const float (&m)[V], const int (&e)[V], const float (&s)[V], const Place<V, WT, GW>& p, float* lds) {
+    constexpr int TG = WT * GW, CW = 64 / GW * V;
 #pragma unroll
-    for (int i = 0; i < V; ++i) A[i] = 1.f, S[i] = 0.f;
-#pragma unroll 4
-    for (int k = lo; k < hi; ++k) {
-        const float* g = agg + 2 * (int64_t)(FWD ? k : lo + hi - 1 - k) * all + chan;
+    for (int i = 0; i < V; ++i) {
+        const int at = p.tg * CW + p.cx * V + i;
+        lds[at] = m[SAME ? 0 : i];
+        lds[TG * CW + at] = __int_as_float(e[SAME ? 0 : i]);
+        lds[2 * TG * CW + at] = s[i];
+    }
+    __syncthreads();
+    Span r{1.f, 0, 0.f};
+    if (p.wave == 0) {
+        static_assert(CW <= 64, "a channel per lane of the first wave");
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const float ak = g[SAME ? 0 : i];
-            S[i] = fmaf(ak, S[i], g[all + i]);
-            A[i] *= ak;
+        for (int g = 0; g < TG; ++g) {
+            const int at = (FWD ? g : TG - 1 - g) * CW + p.lane % CW;
+            r = span_after(Span{lds[at], __float_as_int(lds[TG * CW + at]), lds[2 * TG * CW + at]}, r);
         }
     }
-    join<V, WT, GW, FWD, SAME>(A, S, Ae, Se, At, St, p.lane, p.wave, lds);
+    return r;
 }
 
-// ---- splits: each one's composition (A, S), forwards or backwards --------------------------------------------------------------
-// Every thread walks a stretch of its own (split_len / 16 steps) and the workgroup joins once, so this pass is loads and three operations per element.
+// carry becomes the state behind the splits [s0, s1) of the thread's channels, whose spans are shared out over the time groups (walked forwards or
+// backwards).  agg: per split three planes m, e, s of `all` channels.
+template <int V, int WT, int GW, bool FWD, bool SAME>
+__device__ __forceinline__ void join_splits(const float* __restrict__ agg, int64_t all, int64_t chan, int s0, int s1, const Place<V, WT, GW>& p,
+                                            float (&carry)[V], float* lds) {
+    constexpr int TG = WT * GW, CW = 64 / GW * V;
+    const int q = (s1 - s0 + TG - 1) / TG, lo = min(s1, s0 + p.tg * q), hi = min(s1, lo + q);
+    float m[V], s[V];
+    int e[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) m[i] = 1.f, e[i] = 0, s[i] = 0.f;
+#pragma unroll 4
+    for (int k = lo; k < hi; ++k) {
+        const float* g = agg + 3 * (int64_t)(FWD ? k : lo + hi - 1 - k) * all + chan;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const int o = SAME ? 0 : i;
+            const Span r = span_after(Span{g[o], __float_as_int(g[all + o]), g[2 * all + i]}, Span{m[i], e[i], s[i]});
+            m[i] = r.m, e[i] = r.e, s[i] = r.s;
+        }
+    }
+    const Span r = join_groups<V, WT, GW, FWD, SAME>(m, e, s, p, lds);
+    __syncthreads();
+    if (threadIdx.x < CW) lds[threadIdx.x] = r.m, lds[CW + threadIdx.x] = __int_as_float(r.e), lds[2 * CW + threadIdx.x] = r.s;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const int at = p.cx * V + i;
+        carry[i] = span_apply(Span{lds[at], __float_as_int(lds[CW + at]), lds[2 * CW + at]}, carry[i]);
+    }
+    __syncthreads();                                            // (the slabs' joins use the same memory)
+}
+
+// ---- splits: each one's span, forwards or backwards ---------------------------------------------------------------------------
+// Every thread walks a stretch of its own (split_len / 16 steps) and the workgroup joins once, so this pass is loads and three operations per element
+// (the product's exponent is taken out every eight steps).
 // CN / HAT: how q_check / q_hat are loaded (CN: V elements or one; HAT: 0 no q_hat, 1 V elements, 2 one).
 template <typename D, int V, bool FWD, bool CN, int HAT>
 __global__ __launch_bounds__(256) void recur_split_kernel(const D* __restrict__ in, Gate gc, Gate gh, const int32_t* __restrict__ lengths,
                                                           float* __restrict__ agg, Dims d) {
     constexpr int WT = 4, GW = 4, kU = 8;
     using P = Place<V, WT, GW>;
-    __shared__ float s_join[WT * P::CX * V * 2];
+    __shared__ float s_span[span_floats<V, WT, GW>()];
     const P p(d);
     if (!p.work) return;
     if (p.split == (FWD ? d.splits - 1 : 0)) return;            // (uniform) nothing starts behind the last split
@@ -252,9 +312,14 @@ __global__ __launch_bounds__(256) void recur_split_kernel(const D* __restrict__ 
     const D* pi = in ? in + ((int64_t)p.b * d.T + lo) * C + pc : nullptr;
     const D* pg = static_cast<const D*>(gc.p) + p.b * gc.sb + (int64_t)lo * gc.st + gate_coff(gc, pc, d.N);
     const D* ph = HAT ? static_cast<const D*>(gh.p) + p.b * gh.sb + (int64_t)lo * gh.st + gate_coff(gh, pc, d.N) : nullptr;
-    float A[V], S[V];
+    float A[V], S[V];                                           // (one product for channels that share their gate)
+    int E[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) A[i] = 1.f, S[i] = 0.f;
+    for (int i = 0; i < V; ++i) A[i] = 1.f, E[i] = 0, S[i] = 0.f;
+    auto norm = [&] {
+#pragma unroll
+        for (int i = 0; i < (CN ? V : 1); ++i) span_norm(A[i], E[i]);
+    };
     auto take = [&](const gf_vec<D, V>& ra, const gf_vec<D, V>& rb, const gf_vec<D, V>& rq) {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
@@ -262,7 +327,7 @@ __global__ __launch_bounds__(256) void recur_split_kernel(const D* __restrict__ 
             float b = gf_to_f<D>(rb.e[i]);
             if (HAT) b *= pick<D, V, HAT == 1>(rq, i);
             S[i] = FWD ? fmaf(a, S[i], b) : a * (b + S[i]);
-            A[i] *= a;
+            if (CN || i == 0) A[i] *= a;
         }
     };
     const int n = max(hi - lo, 0), whole = in ? n / kU * kU : 0;
@@ -277,6 +342,7 @@ __global__ __launch_bounds__(256) void recur_split_kernel(const D* __restrict__ 
         }
 #pragma unroll
         for (int e = 0; e < kU; ++e) take(ra[FWD ? e : kU - 1 - e], rb[FWD ? e : kU - 1 - e], rq[FWD ? e : kU - 1 - e]);
+        norm();
     };
     auto one = [&](int k) {
         gf_vec<D, V> ra, rb, rq;
@@ -286,6 +352,7 @@ __global__ __launch_bounds__(256) void recur_split_kernel(const D* __restrict__ 
         load_one<D, V, CN>(reinterpret_cast<const char*>(pg + (int64_t)k * gc.st), ra);
         if (HAT) load_one<D, V, HAT == 1>(reinterpret_cast<const char*>(ph + (int64_t)k * gh.st), rq);
         take(ra, rb, rq);
+        norm();
     };
     if (FWD) {
         for (int k = 0; k < whole; k += kU) eight(k);
@@ -294,12 +361,11 @@ __global__ __launch_bounds__(256) void recur_split_kernel(const D* __restrict__ 
         for (int k = n - 1; k >= whole; --k) one(k);
         for (int k = whole - kU; k >= 0; k -= kU) eight(k);
     }
-    float Ae[V], Se[V], At[V], St[V];
-    join<V, WT, GW, FWD, !CN>(A, S, Ae, Se, At, St, p.lane, p.wave, s_join);
-    if (p.on && p.tg == 0) {
-        float* g = agg + 2 * (int64_t)p.split * all + (int64_t)p.b * d.C + pc;
-#pragma unroll
-        for (int i = 0; i < V; ++i) g[i] = At[i], g[all + i] = St[i];
+    const Span r = join_groups<V, WT, GW, FWD, !CN>(A, E, S, p, s_span);
+    const int c = p.column * P::CW + (int)threadIdx.x;
+    if (threadIdx.x < P::CW && c < d.C) {
+        float* g = agg + 3 * (int64_t)p.split * all + (int64_t)p.b * d.C + c;
+        g[0] = r.m, g[all] = __int_as_float(r.e), g[2 * all] = r.s;
     }
 }
 
@@ -310,7 +376,8 @@ __global__ __launch_bounds__(64 * (WT == 1 ? 4 : WT)) void recur_fwd_kernel(cons
                                                                             float* __restrict__ zT, float* __restrict__ ckpt,
                                                                             float* __restrict__ agg, Dims d) {
     using P = Place<V, WT, GW>;
-    __shared__ float s_join[WT == 1 ? 1 : 2][WT == 1 ? 1 : WT * P::CX * V * 2];
+    constexpr int JOIN = WT == 1 ? 1 : WT * P::CX * V * 2;
+    __shared__ float s_mem[WT == 1 ? 1 : span_floats<V, WT, GW>()];        // the splits' spans, then two joins' buffers
     const P p(d);
     if (!p.work) return;
     int len = d.T;
@@ -328,11 +395,8 @@ __global__ __launch_bounds__(64 * (WT == 1 ? 4 : WT)) void recur_fwd_kernel(cons
 #pragma unroll
         for (int i = 0; i < V; ++i) carry[i] = z0[chan + i];
     }
-    if (p.split > 0) {                                  // (uniform) the splits before this one
-        float At[V], St[V];
-        join_splits<V, WT, GW, true, !CN>(agg, all, chan, 0, p.split, p, At, St, s_join[WT == 1 ? 0 : 1]);
-#pragma unroll
-        for (int i = 0; i < V; ++i) carry[i] = fmaf(At[i], carry[i], St[i]);
+    if constexpr (WT > 1) {
+        if (p.split > 0) join_splits<V, WT, GW, true, !CN>(agg, all, chan, 0, p.split, p, carry, s_mem);     // (uniform) the splits before this one
     }
     const int tbeg = p.split * d.split_len, tend = min(d.T, tbeg + d.split_len);
     const int live_end = min(tend, len);
@@ -382,7 +446,7 @@ __global__ __launch_bounds__(64 * (WT == 1 ? 4 : WT)) void recur_fwd_kernel(cons
                 A[i] *= a[l][i];
             }
         float Ae[V], Se[V], At[V], St[V], h[V];
-        join<V, WT, GW, true, !CN>(A, S, Ae, Se, At, St, p.lane, p.wave, s_join[WT == 1 ? 0 : flip]);
+        join<V, WT, GW, true, !CN>(A, S, Ae, Se, At, St, p.lane, p.wave, s_mem + (WT == 1 ? 0 : flip * JOIN));
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             h[i] = fmaf(Ae[i], carry[i], Se[i]);
@@ -465,7 +529,9 @@ __global__ __launch_bounds__(64 * (WT == 1 ? 4 : WT)) void recur_bwd_kernel(cons
                                                                             const float* __restrict__ ckpt, D* __restrict__ du, GateOut oc, GateOut oh,
                                                                             float* __restrict__ dz0, float* __restrict__ agg, Dims d) {
     using P = Place<V, WT, GW>;
-    __shared__ float s_join[WT == 1 ? 1 : 4][WT == 1 ? 1 : WT * P::CX * V * 2];
+    constexpr int JOIN = WT == 1 ? 1 : WT * P::CX * V * 2;
+    static_assert(WT == 1 || 4 * JOIN <= span_floats<V, WT, GW>(), "four joins' buffers in the memory of the splits' spans");
+    __shared__ float s_mem[WT == 1 ? 1 : span_floats<V, WT, GW>()];
     const P p(d);
     if (!p.work) return;
     int len = d.T;
@@ -488,11 +554,8 @@ __global__ __launch_bounds__(64 * (WT == 1 ? 4 : WT)) void recur_bwd_kernel(cons
 #pragma unroll
         for (int i = 0; i < V; ++i) carry[i] = dzT[chan + i];
     }
-    if (p.split + 1 < d.splits) {                       // (uniform) the splits behind this one
-        float At[V], St[V];
-        join_splits<V, WT, GW, false, !CN>(agg, all, chan, p.split + 1, d.splits, p, At, St, s_join[WT == 1 ? 0 : 2]);
-#pragma unroll
-        for (int i = 0; i < V; ++i) carry[i] = fmaf(At[i], carry[i], St[i]);
+    if constexpr (WT > 1) {                             // (uniform) the splits behind this one
+        if (p.split + 1 < d.splits) join_splits<V, WT, GW, false, !CN>(agg, all, chan, p.split + 1, d.splits, p, carry, s_mem);
     }
     const int tbeg = p.split * d.split_len, tend = min(d.T, tbeg + d.split_len);
     const int slabs = tend > tbeg ? (tend - tbeg + P::SLAB - 1) / P::SLAB : 0;
@@ -548,7 +611,7 @@ __global__ __launch_bounds__(64 * (WT == 1 ? 4 : WT)) void recur_bwd_kernel(cons
                 A[i] *= a[l][i];
             }
         float Ae[V], Re[V], At[V], Rt[V], r[V];
-        join<V, WT, GW, false, !CN>(A, R, Ae, Re, At, Rt, p.lane, p.wave, s_join[WT == 1 ? 0 : flip]);
+        join<V, WT, GW, false, !CN>(A, R, Ae, Re, At, Rt, p.lane, p.wave, s_mem + (WT == 1 ? 0 : flip * JOIN));
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             r[i] = fmaf(Ae[i], carry[i], Re[i]);
@@ -564,7 +627,7 @@ __global__ __launch_bounds__(64 * (WT == 1 ? 4 : WT)) void recur_bwd_kernel(cons
                 for (int l = 0; l < kL; ++l)
 #pragma unroll
                     for (int i = 0; i < V; ++i) S[i] = fmaf(a[l][i], S[i], HAT ? x[l][i] * q[l][i] : x[l][i]);
-                join<V, WT, GW, true, !CN>(A, S, Ae, Se, At, St, p.lane, p.wave, s_join[WT == 1 ? 0 : flip + 1]);
+                join<V, WT, GW, true, !CN>(A, S, Ae, Se, At, St, p.lane, p.wave, s_mem + (WT == 1 ? 0 : (flip + 1) * JOIN));
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
                     const float start = ckpt[((int64_t)p.b * d.nck + ts / d.every) * d.C + pc + i];
@@ -602,7 +665,7 @@ __global__ __launch_bounds__(64 * (WT == 1 ? 4 : WT)) void recur_bwd_kernel(cons
                 if (HAT && oh.mode) put_gate<D, V, P::CX>(oh, oq, soh.at(ts + l), off, tbase + t0 + l, p.on, in, p.lane);
             }
         }
-        flip ^= 2;                                              // (per joined slab: the first one may not meet join_splits' buffer 2 again)
+        flip ^= 2;
     }
     if (p.on && p.tg == 0) {
         if (p.split == 0 && dz0) {
@@ -790,7 +853,7 @@ size_t out_floats(int kind, const Dims& d, const Shape& s) {
     const size_t f = m == kOutTime ? (size_t)wave_columns(d, s) * d.B * d.T : (size_t)d.B * d.T * d.C;
     return (f + 3) / 4 * 4;                                     // the next region starts 16-byte aligned
 }
-size_t agg_floats(const Dims& d) { return d.splits > 1 ? ((size_t)2 * d.splits * d.B * d.C + 3) / 4 * 4 : 0; }
+size_t agg_floats(const Dims& d) { return d.splits > 1 ? ((size_t)3 * d.splits * d.B * d.C + 3) / 4 * 4 : 0; }
 
 template <typename D>
 int forward_t(const Shape& s, const Dims& d, const void* u, Gate gc, Gate gh, const float* z0, const int32_t* lengths, void* z, float* zT, float* ckpt,

@@ -273,7 +273,8 @@ enum { GF_GATE_N = 1, GF_GATE_H = 2, GF_GATE_B = 4 };
  * z0 [B, H, N] fp32 (NULL = 0); lengths [B] int32 on the device (NULL = T; values are clamped to [0, T]): steps at or behind a sequence's
  * length leave the state as it is and give z = 0, whatever they hold.  zT [B, H, N] fp32 is the last state.
  * checkpoints (gf_recurrence_checkpoint_floats, NULL = not kept): one fp32 state every few steps, what the backward pass recomputes the
- * states from.  Products of q_check over a few hundred steps must stay finite in fp32.
+ * states from.  The product of q_check over any 64 consecutive steps must be finite in fp32 (|q_check| < 4 always is); over longer stretches only
+ * the states have to stay in range.
  * Tensors are aligned to four elements.  B >= 1, T >= 0, H N < 2^26; B times the channel chunks (16 to 256 channels) < 2^24. */
 size_t gf_recurrence_checkpoint_floats(int32_t B, int32_t T, int32_t H, int32_t N, int32_t kind_check, int32_t has_hat, int32_t kind_hat);
 size_t gf_recurrence_workspace_bytes(int32_t B, int32_t T, int32_t H, int32_t N, int32_t kind_check, int32_t has_hat, int32_t kind_hat, int32_t backward);

@@ -265,3 +265,47 @@ def test_more_than_two_to_the_31_elements():
 def test_many_sequences():
     ins = make(70000, 3, 1, 1, "time", None, torch.float32, seed=12)
     check(run(*ins[:4], None, *ins[4:]), ins, None, torch.float32)
+
+
+def grown(B, T, H, N, kind, dtype, seed, forward):
+    """Gates whose product over the whole sequence passes the largest float32, with a state (forward: z, else its adjoint) that stays in range: zero or
+    tiny until the last steps of its walk."""
+    g = torch.Generator().manual_seed(seed)
+    q = torch.full(gate_shape(kind, B, T, H, N), 1.0)
+    late = T // 3
+    q[:, :300] = 1.2 + 0.01 * torch.rand(q[:, :300].shape, generator=g)
+    q[:, T - late - 300:T - late] = 1.2 + 0.01 * torch.rand(q[:, T - late - 300:T - late].shape, generator=g)
+    q = q.to(dtype)
+    u, dz = torch.zeros((B, T, H, N)), torch.zeros((B, T, H, N))
+    (u if forward else dz)[:, T - 100:] = torch.randn((B, 100, H, N), generator=g)
+    z0 = torch.where(torch.rand((B, H, N), generator=g) < 0.5, 0.0, 1e-30)
+    if forward:
+        return u.to(dtype), q, None, z0, dz.to(dtype), torch.zeros((B, H, N))
+    return u.to(dtype), q.flip(1), None, torch.zeros((B, H, N)), dz.flip(1).to(dtype), z0
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("shape", [(1, 20000, 2, 4), (3, 2048, 2, 3), (2, 1500, 1, 26)], ids=str)
+@pytest.mark.parametrize("kind", ["full", "node", "feature", "time"])
+@pytest.mark.parametrize("forward", [True, False])
+def test_products_beyond_the_range_of_a_number(shape, kind, forward, dtype):
+    """Splits of the time axis are composed without the product of all their gates having to be a float32: what the step by step walk gives in range
+    is answered in range."""
+    ins = grown(*shape, kind, DT[dtype], sum(shape), forward)
+    check(run(*ins[:4], None, *ins[4:]), ins, None, DT[dtype])
+    lengths = torch.tensor([shape[1] - 50, shape[1], 700][:shape[0]], dtype=torch.int32)
+    check(run(*ins[:4], lengths, *ins[4:]), ins, lengths, DT[dtype])
+
+
+def test_growth_over_the_whole_sequence():
+    B, T, H, N = 1, 20000, 2, 4                                  # 1.01^20000 = 1e86
+    g = torch.Generator().manual_seed(0)
+    u, q, zero = torch.zeros((B, T, H, N)), torch.full((B, T, 1, 1), 1.01), torch.zeros((B, H, N))
+    u[:, T - 100:] = torch.randn((B, 100, H, N), generator=g)
+    dz = torch.zeros_like(u)
+    dz[:, :100] = torch.randn((B, 100, H, N), generator=g)
+    ins = (u, q, None, zero, dz, zero)
+    out = run(*ins[:4], None, *ins[4:])
+    check(out, ins, None, torch.float32)
+    z, zT = linear_recurrence(u.cuda(), q.cuda())                # no initial state: the same walk from zeros
+    assert np.array_equal(z.double().cpu().numpy(), out["z"]) and np.array_equal(zT.double().cpu().numpy(), out["zT"]) and (z[:, :T - 100] == 0).all()
