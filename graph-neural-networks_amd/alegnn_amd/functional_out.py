@@ -11,7 +11,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .functional_seq import _FLOATS, _require_cuda, _same_device
+from .functional_seq import _FLOATS, _no_tangent, _require_cuda, _same_device
 
 TOP_MAX = 64
 _I64 = (torch.int64,)
@@ -32,6 +32,7 @@ def _explain_logits(who, logits, dim, temperature):
 
 def _explain_tokens(logits, tokens, top, temperature, dim):
     who = "token_log_probs"
+    _no_tangent(who, logits=logits)
     V, lead = _explain_logits(who, logits, dim, temperature)
     assert 0 <= top <= min(V, TOP_MAX), f"{who}: top={top} for {V} outputs (want 0..min(V, {TOP_MAX}))"
     assert tuple(tokens.shape) == lead, f"{who}: tokens have shape {tuple(tokens.shape)}, logits {tuple(logits.shape)} with the classes along {dim}"
@@ -42,6 +43,7 @@ def _explain_tokens(logits, tokens, top, temperature, dim):
 
 def _explain_distill(logits, indices, values, temperature, dim):
     who = "distill_top"
+    _no_tangent(who, logits=logits, values=values)
     _, lead = _explain_logits(who, logits, dim, temperature)
     K = indices.shape[-1] if indices.dim() else 0
     assert 1 <= K <= TOP_MAX, f"{who}: indices have shape {tuple(indices.shape)} (want [..., K] with 1 <= K <= {TOP_MAX})"
@@ -65,7 +67,7 @@ def token_log_probs(logits, tokens, top=0, temperature=1.0, ignore_index=-100, e
     in ascending index order.
     A row whose token is `ignore_index` has logp 0 (its entropy and alternatives are answered all the same); any other token outside [0, V)
     gives NaN.  -inf marks an output that is ruled out; a row of nothing else has logp -inf, entropy 0 and gradient 0.  A NaN or +inf logit
-    makes its row's values NaN.  0 <= top <= min(V, 64).  Differentiable (once) in logits through logp, entropy and top_logp."""
+    makes its row's values NaN.  0 <= top <= min(V, 64).  Differentiable (once, in reverse mode) in logits through logp, entropy and top_logp."""
     host = _lib.host()
     top, temperature = int(top), float(temperature)
     try:
@@ -86,7 +88,7 @@ def distill_top(logits, indices, values, temperature=1.0, tail=False, dim=-1):
                   loss = sum_k p_k (log p_k - log q[i_k]) + p_r (log p_r - log q_r), q_r = the mass of the outputs that are not named.
                   (With every output named there are none: the loss is inf if the values leave any mass.)
     A row without entries (tail=False: without mass) has loss 0 and gradient 0; an index that is named twice counts as two entries.  No factor
-    temperature^2 is applied.  Differentiable (once) in logits; the teacher's values are constants."""
+    temperature^2 is applied.  Differentiable (once, in reverse mode) in logits; the teacher's values are constants."""
     host = _lib.host()
     temperature = float(temperature)
     try:

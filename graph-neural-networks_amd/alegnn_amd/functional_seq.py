@@ -8,6 +8,7 @@ one filter per step; the gates are GatedGRNN's q_hat / q_check (time, node) and,
 from __future__ import annotations
 
 import torch
+import torch.autograd.forward_ad as fwAD
 
 from . import _lib
 
@@ -22,6 +23,13 @@ def _require_cuda(who, name, t, dtypes):
                            "CPU fallback; move the data to 'cuda'.")
     if t.dtype not in dtypes:
         raise TypeError(f"alegnn_amd.{who}: `{name}` has dtype {t.dtype}; supported: {', '.join(str(d) for d in dtypes)}")
+
+
+def _no_tangent(who, **inputs):
+    """Forward-mode derivatives are not there: a tangent is refused, not dropped."""
+    for name, t in inputs.items():
+        if t is not None and t.is_floating_point() and fwAD.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"alegnn_amd.{who}: `{name}` carries a tangent; forward-mode derivatives are not supported")
 
 
 def _same_device(who, name, t, x):
@@ -39,6 +47,7 @@ def _check_gate(who, q, shape, name):
 def _explain(u, q_check, q_hat, z0, lengths):
     """Why the arguments were refused."""
     who = "linear_recurrence"
+    _no_tangent(who, u=u, q_check=q_check, q_hat=q_hat, z0=z0)
     assert u.dim() == 4, f"{who}: u has shape {tuple(u.shape)}, want [B, T, H, N]"
     _require_cuda(who, "u", u, _FLOATS)
     assert max(u.shape) <= 2 ** 31 - 2 ** 17, f"{who}: u has shape {tuple(u.shape)}: a side over 2^31 - 2^17"
@@ -67,7 +76,7 @@ def linear_recurrence(u, q_check, q_hat=None, z0=None, lengths=None):
     gradient.  Returns z [B,T,H,N] in u's dtype and the last state zT [B,H,N] in float32 -- what the next call takes as z0, so a sequence can
     be fed in pieces down to single steps (T = 1) without losing the state's precision.  The state is float32 throughout; the product of
     q_check over any 64 consecutive steps must be finite (gates below 4 in magnitude always are), over longer stretches only the states have
-    to stay in range.  Differentiable (once) in u, q_check, q_hat and z0."""
+    to stay in range.  Differentiable (once, in reverse mode) in u, q_check, q_hat and z0."""
     host = _lib.host()
     try:
         return host.linear_recurrence(u, q_check, q_hat, z0, lengths)

@@ -48,6 +48,11 @@ void want(bool ok) {
     if (!ok) throw Refused();
 }
 
+// Forward-mode derivatives: a dual tensor does not require a gradient, so the direct path would answer without its tangent.
+void no_tangent(std::initializer_list<Tensor> inputs) {
+    for (const Tensor& t : inputs) want(!t.defined() || !t._fw_grad(/*level=*/0).defined());
+}
+
 int dtype_of(const Tensor& t) {
     switch (t.scalar_type()) {
         case at::kFloat: return GF_F32;
@@ -156,6 +161,7 @@ std::tuple<Tensor, Tensor> linear_recurrence(const Tensor& u, const Tensor& qc, 
                                              const std::optional<Tensor>& lengths_) {
     const Tensor qh = qh_.value_or(Tensor()), z0 = z0_.value_or(Tensor());
     Tensor lengths = lengths_.value_or(Tensor());
+    no_tangent({u, qc, qh, z0});
     want(u.dim() == 4 && u.is_cuda() && dtype_of(u) >= 0);
     for (const int64_t n : u.sizes()) want(n <= (1ll << 31) - (1ll << 17));
     Kinds k{0, 0, qh.defined()};
@@ -267,6 +273,7 @@ struct TokenLogProbs : torch::autograd::Function<TokenLogProbs> {
 
 py::tuple token_log_probs(const Tensor& logits, Tensor tokens, int64_t top, double temperature, int64_t ignore, bool entropy, int64_t dim) {
     std::vector<int64_t> lead;
+    no_tangent({logits});
     const Tensor x = rows_of(logits, dim, lead);
     want(usable(temperature) && top >= 0 && top <= 64 && top <= x.size(1));
     want(tokens.sizes() == at::IntArrayRef(lead) && tokens.scalar_type() == at::kLong && tokens.device() == x.device());
@@ -332,6 +339,7 @@ struct DistillTop : torch::autograd::Function<DistillTop> {
 
 Tensor distill_top(const Tensor& logits, Tensor indices, Tensor values, double temperature, bool tail, int64_t dim) {
     std::vector<int64_t> lead;
+    no_tangent({logits, values});
     const Tensor x = rows_of(logits, dim, lead);
     want(usable(temperature) && indices.dim() == (int64_t)lead.size() + 1);
     const int64_t K = indices.size(-1);

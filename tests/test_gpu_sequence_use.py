@@ -331,3 +331,27 @@ def test_backward_captured_from_detached_leaves_while_an_eager_graph_lives():
         wends, wgrads = body()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip([*ends, *grads], [*wends, *wgrads])), i
+
+
+def test_forward_mode_derivatives_are_refused():
+    """A tangent is not dropped without a word, whichever input carries it."""
+    import torch.autograd.forward_ad as fwAD
+    u, q = torch.randn(2, 5, 3, 4, device="cuda"), torch.rand(2, 5, 3, 4, device="cuda")
+    z0, x, t, v = torch.randn(2, 3, 4, device="cuda"), torch.randn(3, 7, device="cuda"), torch.tensor([0, 3, 6], device="cuda"), torch.zeros(3, 1, device="cuda")
+    with fwAD.dual_level():
+        def dual(a):
+            return fwAD.make_dual(a, torch.ones_like(a))
+        for grad in (False, True):
+            u, x = u.detach().requires_grad_(grad), x.detach().requires_grad_(grad)
+            for call in (lambda: linear_recurrence(dual(u), q), lambda: linear_recurrence(u, dual(q)), lambda: linear_recurrence(u, q, dual(q)),
+                         lambda: linear_recurrence(u, q, q, dual(z0)), lambda: token_log_probs(dual(x), t), lambda: distill_top(dual(x), t[:, None], v),
+                         lambda: distill_top(x, t[:, None], dual(v)), lambda: token_log_probs(dual(x).t(), t, dim=0)):
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    call()
+        linear_recurrence(u, q, q, z0), token_log_probs(x, t), distill_top(x, t[:, None], v)      # no tangent: served as ever
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda a: token_log_probs(a, t)[0], (x.detach(),), (torch.ones_like(x),))
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(lambda a: linear_recurrence(a[None], q[:1])[0])(u.detach())
+    with pytest.raises(RuntimeError):
+        torch.func.grad(lambda a: distill_top(a, t[:, None], v).sum())(x.detach())

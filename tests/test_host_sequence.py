@@ -216,3 +216,19 @@ def test_restatement_of_tokens_and_distillation_against_autograd():
         out, _ = ref.distill(x.numpy(), idx.numpy(), val.numpy(), 2.0, tail, np.ones(R), (0.0, 0.0))
         assert np.allclose(out["loss"][:3], [float(v) for v in rows], rtol=1e-10) and out["loss"][3] == 0
         assert np.allclose(out["dlogits"], d.numpy(), rtol=1e-9, atol=1e-12)
+
+
+def test_a_tangent_is_named_before_anything_else_is():
+    import torch.autograd.forward_ad as fwAD
+    u, x, t, v = torch.zeros(2, 3, 4, 5), torch.zeros(3, 7), torch.zeros(3, dtype=torch.int64), torch.zeros(3, 1)
+    with fwAD.dual_level():
+        def dual(a):
+            return fwAD.make_dual(a, torch.ones_like(a))
+        for name, call in (("u", lambda: linear_recurrence(dual(u), u)), ("q_check", lambda: linear_recurrence(u, dual(u))),
+                           ("q_hat", lambda: linear_recurrence(u, u, dual(u))), ("z0", lambda: linear_recurrence(u, u, u, dual(u[:, 0]))),
+                           ("logits", lambda: token_log_probs(dual(x), t)), ("logits", lambda: distill_top(dual(x), t[:, None], v)),
+                           ("values", lambda: distill_top(x, t[:, None], dual(v)))):
+            with pytest.raises(NotImplementedError, match=f"`{name}` carries a tangent"):
+                call()
+        with pytest.raises(RuntimeError, match="no CPU fallback"):
+            linear_recurrence(u, u)
