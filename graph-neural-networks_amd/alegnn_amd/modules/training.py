@@ -19,8 +19,8 @@ checkpoints are written by rank 0 (model.py).
 ``teacherTop=(classes, logProbs)`` (superset option): two [nTrain, K] tensors, the K best classes of a teacher for every training sample with
 their log probabilities (evaluation.predictTop of the training split, K <= 64, an index outside the classes = padding).  A step then minimises
 (1 - distillWeight) * loss + distillWeight * mean distill_top(output, classes, logProbs) with what the K classes leave as one further outcome
-(distillWeight 0.5, distillTemperature 1.0: the temperature the log probabilities were taken at).  With as many entries as classes there is no
-further outcome: the entries' probabilities are then scaled to one.  Validation keeps the plain loss.
+(distillWeight 0.5, distillTemperature 1.0: the temperature the log probabilities were taken at).  A sample whose entries name every class has no
+further outcome: their probabilities are then scaled to one.  Validation keeps the plain loss.
 
 ``hipGraph=True`` (superset option, GPU only): zero-grad + forward + loss + backward of a training step are captured once per
 batch size as a HIP graph and replayed; the samples are copied into the graph's static input buffers, the (all-reduce and)
@@ -47,6 +47,12 @@ def _world():
     if dist.is_available() and dist.is_initialized():
         return dist.get_rank(), dist.get_world_size()
     return 0, 1
+
+
+def _names_all(classes, C):
+    """Which rows of [n, K] entries name every one of C classes."""
+    spot = torch.where((classes >= 0) & (classes < C), classes, C)
+    return torch.zeros((classes.shape[0], C + 1), dtype=torch.bool, device=classes.device).scatter_(1, spot, True)[:, :C].all(1)
 
 
 class Trainer:
@@ -107,6 +113,7 @@ class Trainer:
             if classes.shape != logProbs.shape or classes.dim() != 2 or classes.shape[0] != nTrain:
                 raise ValueError(f"teacherTop: two [nTrain, K] tensors wanted, got {tuple(classes.shape)} and {tuple(logProbs.shape)} for nTrain = {nTrain}")
             self.teacher = (classes.detach().to(torch.int64), logProbs.detach().float())
+            self._teacherWhole = {}                                 # number of classes: whether every sample's entries name them all
             self.distillWeight = float(kwargs.get('distillWeight', 0.5))
             self.distillTemperature = float(kwargs.get('distillTemperature', 1.0))
             if not 0.0 <= self.distillWeight <= 1.0:
@@ -143,10 +150,17 @@ class Trainer:
             return lossValue
         w, tau = self.distillWeight, self.distillTemperature
         classes, logProbs = teacher
-        tail = classes.shape[1] < yHat.shape[-1]
-        if not tail:                                                # every class is named: what rounding leaves to one belongs to none
-            logProbs = logProbs * tau
-        return (1.0 - w) * lossValue + w * distill_top(yHat, classes, logProbs, temperature=tau, tail=tail).mean()
+        C = yHat.shape[-1]
+        if C not in self._teacherWhole:                             # (once, in a step that is not captured)
+            self._teacherWhole[C] = classes.shape[1] >= C and bool(_names_all(self.teacher[0], C).all())
+        # every class named: what rounding leaves to one belongs to none, and the entries are scaled instead (their logits are logProbs * tau)
+        if self._teacherWhole[C]:
+            loss = distill_top(yHat, classes, logProbs * tau, temperature=tau)
+        else:
+            loss = distill_top(yHat, classes, logProbs, temperature=tau, tail=True)
+            if classes.shape[1] >= C:                               # some samples name them all, some do not
+                loss = torch.where(_names_all(classes, C), distill_top(yHat, classes, logProbs * tau, temperature=tau), loss)
+        return (1.0 - w) * lossValue + w * loss.mean()
 
     # ---- the step as a HIP graph (hipGraph=True) ---------------------------------------------------------------------
     def _graph_step(self, xTrain, yTrain, samplesType, indices, weight):

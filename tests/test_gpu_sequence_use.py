@@ -355,3 +355,43 @@ def test_forward_mode_derivatives_are_refused():
         torch.func.vmap(lambda a: linear_recurrence(a[None], q[:1])[0])(u.detach())
     with pytest.raises(RuntimeError):
         torch.func.grad(lambda a: distill_top(a, t[:, None], v).sum())(x.detach())
+
+
+def test_a_student_of_padded_entries(tmp_path):
+    """As many entries as classes or more, some of them padding: a row that names every class has no further outcome, one that does not keeps it."""
+    S = gso(30, 3).astype(np.float32)
+    data = Data(30)
+    teacher = model_of(S, 0, tmp_path, "pad-teacher")
+    ans = predictTop(teacher, data, 'train', top=5, temperature=2.0)
+    classes = torch.cat((ans['topClasses'], torch.full((data.nTrain, 2), -1, device="cuda")), 1)
+    values = torch.cat((ans['topLogProb'], torch.zeros(data.nTrain, 2, device="cuda")), 1)
+    classes[::3, 2:5] = -1                                          # two named classes
+    classes[1::9] = -1                                              # no teacher at all
+    classes[2, 5], values[2, 5] = 99, 0.5                           # padding on the other side
+    losses, ends = [], []
+    for graph in (False, True):                                     # eagerly, and eight replays of a graph
+        np.random.seed(1)
+        student = model_of(S, 7, tmp_path, "pad-student%d" % graph)
+        v = student.train(data, 2, 16, printInterval=0, validationInterval=100, teacherTop=(classes, values), distillWeight=1.0, distillTemperature=2.0,
+                          hipGraph=graph)
+        losses.append(v['lossTrain'])
+        ends.append([p.detach().clone() for p in student.archit.parameters()])
+        assert np.isfinite(v['lossTrain']).all() and all(torch.isfinite(q).all() for q in ends[-1])
+    assert np.allclose(losses[0], losses[1], rtol=1e-6) and all(torch.equal(a, b) for a, b in zip(*ends))
+    np.random.seed(1)                                               # the first step by hand
+    student = model_of(S, 7, tmp_path, "pad-hand")
+    first = np.random.permutation(data.nTrain)[:16]
+    with torch.no_grad():
+        lq = torch.log_softmax(student.archit(data.parts['train'][0][first].cuda()).double().cpu() / 2.0, 1)
+        lp = torch.log_softmax(teacher.archit(data.parts['train'][0][first].cuda()).double().cpu() / 2.0, 1)
+    want = 0.0
+    for r, c in enumerate(classes.cpu()[first]):
+        c = c[(c >= 0) & (c < 5)]
+        if len(c):
+            want += float((lp[r, c].exp() * (lp[r, c] - lq[r, c])).sum())
+            rest = torch.ones(5, dtype=torch.bool)
+            rest[c] = False
+            if rest.any():
+                pr, qr = lp[r, rest].exp().sum(), lq[r, rest].exp().sum()
+                want += float(pr * (pr / qr).log())
+    assert abs(losses[0][0] - want / 16) < 1e-4
