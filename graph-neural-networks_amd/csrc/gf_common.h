@@ -162,6 +162,7 @@ struct gf_tuning {
                                 // next XCC (a 33 / 31 census), 3 = one workgroup never arrives (the others run into the time limit: the slot is poisoned)
     int spmm_tmo_ms = 0;        // MFMA sweep, experiments: time limit of the census / the barriers in ms (0 = 2000)
     int spmm_trace = 0;         // MFMA sweep, experiments: record phase time stamps (gf_debug_msweep_trace)
+    int spmm_cooperr = 0;       // tests: the cooperative launch of a fused chain fails with this hipError_t (nothing is launched)
     int spmm_fuse = 1;          // MFMA sweep: the K - 1 hops of gf_khop in one launch, entry by entry (0 = one launch per hop)
     int spmm_depth = 0;         // MFMA sweep: gathers in flight per wave, 0 = default (10 from 15 sets per wave on, 5 at 10 sets), 5
     int spmm_srcmask = 0;       // MFMA sweep, timing experiments only (results wrong): AND mask on the gathered source offsets (confines them to a window)

@@ -52,7 +52,8 @@ constexpr int kMsCensusWord = 8 * kMsGateWords;
 constexpr int kMsSlotWords = kMsCensusWord + 64;
 enum : int { kCsCount = 0 /* [8] workgroups per XCC */, kCsArrive = 8, kCsGen = 9 /* += 2 per launch; bit 0 = this launch is abandoned */,
              kCsRepair = 10 /* read by the repair kernel behind the launch */, kCsPoison = 11 /* sticky: a launch on this slot timed out */ };
-enum : unsigned { kMsStatusCensus = 1u /* a census did not show 8 x 32 */, kMsStatusTimeout = 2u /* a grid did not become resident / a barrier did not open */ };
+enum : unsigned { kMsStatusCensus = 1u /* a census did not show 8 x 32 */, kMsStatusTimeout = 2u /* a grid did not become resident / a barrier did not open */,
+                 kMsStatusNoCoop = 4u /* host only: no cooperative queue */ };
 
 __device__ __forceinline__ unsigned ag_load(unsigned* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 __device__ __forceinline__ void ag_store(unsigned* p, unsigned v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
@@ -781,6 +782,7 @@ int slot_of(hipStream_t st) {
 // creation (gf_msweep_status_word), never during a launch (a launch may be under stream capture).
 std::atomic<unsigned*> g_status{nullptr};
 std::atomic<int> g_fuse_off{0};   // 1 = a repair was seen (or GFHIP_MSWEEP_FUSE=0): gf_khop runs one launch per hop from here on
+std::atomic<int> g_no_coop{0};    // 1 = the runtime had no cooperative queue to give (g_fuse_off is set with it)
 
 }  // namespace
 
@@ -815,7 +817,7 @@ bool gf_msweep_fusion_allowed() {
 
 extern "C" int gf_msweep_status(uint32_t* flags, int32_t* fusion_on) {
     const unsigned* w = g_status.load();
-    if (flags) *flags = w ? *reinterpret_cast<const volatile unsigned*>(w) : 0u;
+    if (flags) *flags = (w ? *reinterpret_cast<const volatile unsigned*>(w) : 0u) | (g_no_coop.load() ? kMsStatusNoCoop : 0u);
     if (fusion_on) *fusion_on = gf_msweep_fusion_allowed() ? 1 : 0;
     return GF_OK;
 }
@@ -824,6 +826,7 @@ void gf_msweep_status_reset() {   // experiments (gf_tune("spmm_status_reset", 1
     unsigned* w = g_status.load();
     if (w) *reinterpret_cast<volatile unsigned*>(w) = 0u;
     g_fuse_off.store(0);
+    g_no_coop.store(0);
 }
 
 bool gf_msweep_applicable(const gf_csr_dev& m, int N, int B, int W) {
@@ -898,7 +901,9 @@ int gf_msweep_launch(const gf_csr_dev& m, const float* Xin, float* Xtaps, int64_
         else if (deep) GF_MS_P(SV, UV, 10);           \
         else GF_MS_P(SV, UV, 5);                      \
     } while (0)
-    if (m.ms_uniform) {
+    if (chained && g_tune.spmm_cooperr) {
+        lerr = (hipError_t)g_tune.spmm_cooperr;
+    } else if (m.ms_uniform) {
         switch (m.ms_sets) {
             case 10: if (wide) GF_MS(10, 1, 0, 5, 1); else GF_MS_P(10, 1, 5); break;
             case 15: GF_MS_D(15, 1); break;
@@ -917,15 +922,18 @@ int gf_msweep_launch(const gf_csr_dev& m, const float* Xin, float* Xtaps, int64_
 #undef GF_MS_P
 #undef GF_MS
 #undef GF_MSH
-    if (chained && lerr != hipSuccess) {
-        // The runtime has no cooperative queue to give (another process of this GPU holds the only one): nothing was launched.  The process goes on
-        // with one launch per hop -- the same bits -- and the callers run this chain that way.
+    if (chained && lerr == hipErrorIllegalState) {
+        // The runtime has no cooperative queue to give (another process of this GPU holds the only one; "the operation cannot be performed in the
+        // present state"): nothing was launched.  The process goes on with one launch per hop -- the same bits -- and the callers run this chain that
+        // way.  Any other error is the caller's.
         (void)hipGetLastError();
+        g_no_coop.store(1);
         if (!g_fuse_off.exchange(1))
             fprintf(stderr, "gfhip: no cooperative launch for a fused K-hop chain (%s); the chain runs one launch per hop from here on\n", hipGetErrorString(lerr));
         gf_set_error("cooperative launch of spmm_msweep_kernel: %s", hipGetErrorString(lerr));
         return GF_ERR_UNSUPPORTED;
     }
+    GF_HIP(lerr);
     GF_LAUNCH_CHECK("spmm_msweep_kernel");
     if (chained && !a_nostore && src_mask == 0xffffffffu) {
         hipLaunchKernelGGL(spmm_msweep_repair_kernel, dim3((unsigned)(B < 512 ? B : 512)), dim3(512), 0, st, gate + kMsCensusWord, m.rowptr, m.col, m.val, m.rowid,

@@ -85,6 +85,7 @@ extern "C" int gf_tune(const char* key, int32_t value) {
     else if (!strcmp(key, "spmm_pfd")) g_tune.spmm_pfd = value;
     else if (!strcmp(key, "spmm_depth")) g_tune.spmm_depth = value;
     else if (!strcmp(key, "spmm_fuse")) g_tune.spmm_fuse = value;
+    else if (!strcmp(key, "spmm_cooperr")) g_tune.spmm_cooperr = value;
     else if (!strcmp(key, "spmm_trace")) g_tune.spmm_trace = value;
     else if (!strcmp(key, "spmm_xlayout")) g_tune.spmm_xlayout = value;
     else if (!strcmp(key, "spmm_hublim")) g_tune.spmm_hublim = value;

@@ -253,9 +253,9 @@ int gf_spmm_hop_kernel(const gf_plan* plan, int32_t op, int32_t B, int32_t W);
 /* State of the fused chains of this process (no reference counterpart).  A fused launch opens with a census of its workgroups (32 on each of
  * 8 XCCs, all resident); a launch whose census fails, or that runs into its time limit, stores nothing, and the repair kernel queued behind it
  * recomputes the chain with the same bits -- no trap, no wrong result, no host synchronisation.  flags: bit 0 = a census failed, bit 1 = a
- * time limit expired (since the process started); fusion_on = 0 once that has been seen by the host (gf_khop then runs one launch per hop)
- * or when GFHIP_MSWEEP_FUSE=0 is set in the environment, or when the runtime refused a cooperative launch (another process on this GPU
- * holds the cooperative queue). */
+ * time limit expired, bit 2 = the runtime had no cooperative queue to give, as another process on this GPU holds it (since the process started; any
+ * other error of the launch is returned as it is); fusion_on = 0 once one of them has been seen by the host (gf_khop then runs one launch per hop)
+ * or when GFHIP_MSWEEP_FUSE=0 is set in the environment. */
 int gf_msweep_status(uint32_t* flags, int32_t* fusion_on);
 int gf_time_khop(const gf_plan* const* plans, int32_t E, int32_t op, float* Z, int32_t B, int32_t W, int32_t K, int32_t iters,
                  void* stream, float* avg_ms);   /* the same for one gf_khop call (the K-1 hops of every edge feature on a tap stack) */
@@ -275,7 +275,8 @@ enum { GF_GATE_N = 1, GF_GATE_H = 2, GF_GATE_B = 4 };
  * checkpoints (gf_recurrence_checkpoint_floats, NULL = not kept): one fp32 state every few steps, what the backward pass recomputes the
  * states from.  The product of q_check over any 64 consecutive steps must be finite in fp32 (|q_check| < 4 always is); over longer stretches only
  * the states have to stay in range.
- * Tensors are aligned to four elements.  B >= 1, T >= 0, H N < 2^26; B times the channel chunks (16 to 256 channels) < 2^24. */
+ * Tensors are aligned to four elements.  B >= 1, T >= 0, H N < 2^26; B times the channel chunks (of 16 to 1024 channels)
+ * times the splits of the time axis < 2^24. */
 size_t gf_recurrence_checkpoint_floats(int32_t B, int32_t T, int32_t H, int32_t N, int32_t kind_check, int32_t has_hat, int32_t kind_hat);
 size_t gf_recurrence_workspace_bytes(int32_t B, int32_t T, int32_t H, int32_t N, int32_t kind_check, int32_t has_hat, int32_t kind_hat, int32_t backward);
 int gf_recurrence_forward(const void* u, const void* q_check, int32_t kind_check, const void* q_hat, int32_t kind_hat, const float* z0,
@@ -326,7 +327,8 @@ int gf_distill_top_backward(const void* logits, int64_t row_stride, const int64_
  * prefetch lead in loop iterations: 0 = auto from the image's rounds, -1 = off), "spmm_depth" (0 = 10 gathers in flight | 5), "spmm_slack" / "spmm_passes" (image: rounds
  * beyond the mean group length in percent, passes allowed per batch entry; read by gf_plan_create), timing-only: "spmm_srcmask",
  * "spmm_trace"; tests of the abandon-and-repair path: "spmm_census" (1 = census called bad | 2 = one workgroup claims the next XCC |
- * 3 = one workgroup never arrives), "spmm_tmo_ms" (time limit of census / barriers, 0 = 2000), "spmm_status_reset"; "spmm_xlayout" (0/1 the boundary layout pass
+ * 3 = one workgroup never arrives), "spmm_tmo_ms" (time limit of census / barriers, 0 = 2000), "spmm_status_reset"; "spmm_cooperr" (the
+ * cooperative launch of a fused chain fails with this hipError_t, nothing is launched); "spmm_xlayout" (0/1 the boundary layout pass
  * inside the fused chain launch), "spmm_hublim" (image: rows longer than this are hub rows, 0 = the builder's cost model; read by gf_plan_create); "spmm_minwork" (fewest (batch entry,
  * 32-column slab) pairs the sweep takes, default 5: below, SELL-8 is faster); "spmm_xcd" (0/1),
  * "spmm_group" (0/1 locality groups in the row schedule of graphs with N >= 32768; read by gf_plan_create),

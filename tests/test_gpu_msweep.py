@@ -445,3 +445,52 @@ def test_work_lists_of_five_to_seven_pairs_run_as_the_sweep(graph, n, B, W, K, k
             else:
                 assert float((got - sell).abs().max()) <= 1e-5 * float(sell.abs().max()), (op, kw)
         tune(spmm_census=0, spmm_status_reset=1)
+
+
+@pytest.fixture
+def coop_error():
+    yield lambda code: tune(spmm_cooperr=code)
+    tune(spmm_cooperr=0, spmm_status_reset=1)
+
+
+def test_chain_without_a_cooperative_queue_runs_one_launch_per_hop(knobs, coop_error):
+    """hipErrorIllegalState is what the runtime answers where another process holds the cooperative queue (the launch wrapper is told to answer it here,
+    nothing is launched): the chain, and a layer with its layout pass, come out with the same bits, and the state is reported."""
+    from alegnn_amd import LSIGF
+    n, B, K = 60000, 16, 4
+    gso = SparseGSO([er(n, 4, seed=61)])
+    plans = gso.plans(DEV)
+    x0 = torch.randn(B, n, 32, device=DEV)
+    h, x = torch.randn(32, 1, K, 32, device=DEV), torch.randn(B, 32, n, device=DEV)
+    tune(spmm_algo=0, spmm_fuse=1, spmm_status_reset=1)
+    ref = [khop_chain(plans, x0, K, op) for op in (0, 1)]
+    with torch.no_grad():
+        y = LSIGF(h, gso, x)
+    assert chain_status() == (0, 1)
+    for op in (0, 1):
+        coop_error(401)
+        for _ in range(2):                                  # the refused launch, and the calls behind it that do not try again
+            assert torch.equal(khop_chain(plans, x0, K, op), ref[op])
+            assert chain_status() == (4, 0)
+        tune(spmm_status_reset=1)
+    with torch.no_grad():
+        assert torch.equal(LSIGF(h, gso, x), y)
+    assert chain_status() == (4, 0)
+    coop_error(0)
+    tune(spmm_status_reset=1)
+    assert torch.equal(khop_chain(plans, x0, K), ref[0]) and chain_status() == (0, 1)
+
+
+def test_other_errors_of_the_cooperative_launch_are_the_callers(knobs, coop_error):
+    n, B, K = 60000, 16, 4
+    gso = SparseGSO([er(n, 4, seed=61)])                    # (owns its plans)
+    plans = gso.plans(DEV)
+    Z = torch.zeros(K, B, n, 32, device=DEV)
+    tune(spmm_algo=0, spmm_fuse=1, spmm_status_reset=1)
+    L = _lib.lib()
+    for code, word in ((2, b"out of memory"), (720, b"cooperative launch")):
+        coop_error(code)
+        assert L.gf_khop(plans, 1, 0, Z.data_ptr(), B, 32, K, stream()) == -3 and word in L.gf_last_error()
+        assert chain_status() == (0, 1)                     # the next call tries again
+    coop_error(0)
+    assert L.gf_khop(plans, 1, 0, Z.data_ptr(), B, 32, K, stream()) == 0
