@@ -395,3 +395,33 @@ def test_more_rows_than_one_launch_takes(V, dtype):
     want, tol = ref.distill(xs, idx[rows].cpu().numpy(), val[rows].double().cpu().numpy(), 1.0, False, one, half(DT[dtype]))
     within(loss[rows], want["loss"], tol["loss"], "loss")
     within(dd[rows], want["dlogits"], tol["dlogits"], "dlogits")
+
+
+MANY = [(1100, 4099), (700, 10001), (600, 20011)]                   # enough tiles for the largest ones: one, two and three a row in 16 bits
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("size", MANY, ids=str)
+@pytest.mark.parametrize("top", [0, 8])
+def test_tokens_many_rows(size, dtype, top):
+    R, V = size
+    x, g = logits_of(R, V, DT[dtype], R + V)
+    x[:, torch.randperm(V, generator=g)[: V // 10]] = NINF
+    x[0] = NINF
+    tok = x.float().argmax(1)                                       # a given output that is not ruled out, some rows without one
+    tok[5:] = torch.where(torch.isinf(x[5:].gather(1, torch.arange(5, R)[:, None])[:, 0]), tok[5:], torch.arange(5, R))
+    tok[3::17] = -100
+    check_tokens(x, tok, top, T=1.5, seed=V)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("size", MANY, ids=str)
+@pytest.mark.parametrize("tail", [False, True])
+def test_distill_many_rows(size, dtype, tail):
+    R, V = size
+    x, g = logits_of(R, V, DT[dtype], R + V + 1)
+    idx, val = teacher(x, 64, g)
+    idx[torch.rand((R, 64), generator=g) < 0.1] = -1
+    idx[2::19] = -1
+    idx[4, 7] = idx[4, 9]
+    check_distill(x, idx, val, 2.0, tail, seed=V)

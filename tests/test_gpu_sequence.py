@@ -309,3 +309,23 @@ def test_growth_over_the_whole_sequence():
     check(out, ins, None, torch.float32)
     z, zT = linear_recurrence(u.cuda(), q.cuda())                # no initial state: the same walk from zeros
     assert np.array_equal(z.double().cpu().numpy(), out["z"]) and np.array_equal(zT.double().cpu().numpy(), out["zT"]) and (z[:, :T - 100] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("shape", [(2, 31, 5, 52), (3, 29, 3, 51), (2, 30, 2, 130)], ids=str)
+@pytest.mark.parametrize("kc,kh", [("full", "full"), ("node", "full"), ("feature", "node"), ("time", None), ("time1", "time")])
+@pytest.mark.parametrize("padded", [False, True])
+def test_waves_side_by_side_over_more_than_one_slab(shape, kc, kh, padded, dtype):
+    """17 to 32 steps: a workgroup's waves stand side by side along the channels and walk two slabs of 16 steps (the form of many channels)."""
+    ins = make(*shape, kc, kh, DT[dtype], seed=sum(shape) + 2)
+    lengths = torch.tensor([shape[1] - 2, 9, 16][:shape[0]], dtype=torch.int32) if padded else None
+    check(run(*ins[:4], lengths, *ins[4:]), ins, lengths, DT[dtype])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("kc,kh", [("full", "full"), ("node", "time"), ("feature", None)])
+def test_many_channels_and_unlike_lengths(kc, kh, dtype):
+    B, T, H, N = 16, 70, 8, 600                                  # 19200 threads' channels: five slabs, several chunks of channels
+    ins = make(B, T, H, N, kc, kh, DT[dtype], seed=21)
+    lengths = torch.tensor([0, 1, 15, 16, 17, 31, 32, 33, 48, 50, 63, 64, 65, 69, 70, 70], dtype=torch.int32)
+    check(run(*ins[:4], lengths, *ins[4:]), ins, lengths, DT[dtype])
