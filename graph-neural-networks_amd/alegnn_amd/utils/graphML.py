@@ -488,18 +488,30 @@ class HiddenState(nn.Module):
         return reprString
 
 
+def _live_steps(x, lengths):
+    """x [B,T,F,N] with zeros in the steps that do not count: a filter would carry what they hold (NaN, inf) into its taps' gradient."""
+    if lengths is None:
+        return x
+    live = torch.arange(x.shape[1], device=x.device) < lengths[:, None]
+    return torch.where(live[:, :, None, None], x, 0.0)
+
+
+def _linear_grnn(a, gso, x, z0, sigma, q_hat, q_check, xBias, lengths):
+    H, F = a.shape[0], a.shape[3]
+    B, T, N = x.shape[0], x.shape[1], gso.N
+    assert x.shape[2] == F and x.shape[3] == N
+    Ax = LSIGF(a, gso, x.reshape(B * T, F, N), xBias).reshape(B, T, H, N)
+    return linear_recurrence(Ax if sigma is None else sigma(Ax), q_check, q_hat, z0, lengths)
+
+
 def LinearGRNN(a, S, x, z0, sigma, q_hat, q_check, xBias=None, lengths=None):
     """Hidden states z_t = q_check_t * z_{t-1} + q_hat_t * sigma(A(S) x_t), t = 1..T: GatedGRNN (graphML.py:1292-1527) with a state that is carried
     by its gate alone, so that all T steps run in parallel (two launches instead of a filter per step).
 
     a [H,E,K,F] input-to-hidden taps, S the GSO, x [B,T,F,N], z0 [B,H,N] or None, gates [B|1, T, H|1, N|1] (q_hat None = 1), xBias [H,1];
-    lengths [B] int32 = steps of each sequence that count (None = all).  Returns (z [B,T,H,N], z_T [B,H,N])."""
-    H, E, K, F = a.shape
-    gso = SparseGSO.from_any(S)
-    B, T, N = x.shape[0], x.shape[1], gso.N
-    assert x.shape[2] == F and x.shape[3] == N
-    Ax = LSIGF(a, gso, x.reshape(B * T, F, N), xBias).reshape(B, T, H, N)
-    return linear_recurrence(Ax if sigma is None else sigma(Ax), q_check, q_hat, z0, lengths)
+    lengths [B] int32 = steps of each sequence that count (None = all; what the others hold does not matter).  Returns
+    (z [B,T,H,N], z_T [B,H,N])."""
+    return _linear_grnn(a, SparseGSO.from_any(S), _live_steps(x, lengths), z0, sigma, q_hat, q_check, xBias, lengths)
 
 
 class LinearHiddenState(nn.Module):
@@ -557,10 +569,11 @@ class LinearHiddenState(nn.Module):
         assert len(x.shape) == 4 and x.shape[2] == self.F
         B, T, N = x.shape[0], x.shape[1], x.shape[3]
         assert z0 is None or (len(z0.shape) == 3 and z0.shape[0] == B and z0.shape[1] == self.H and z0.shape[2] == N)
+        x = _live_steps(x, lengths)
         flat = x.reshape(B * T, self.F, N)
         i = torch.sigmoid(self.inputGate(flat)).reshape(B, T, -1, N)
         f = torch.sigmoid(self.forgetGate(flat)).reshape(B, T, -1, N)
-        z, zT = LinearGRNN(self.aWeights, self._gso, x, z0, self.sigma, i, f, xBias=self.xBias, lengths=lengths)
+        z, zT = _linear_grnn(self.aWeights, self._gso, x, z0, self.sigma, i, f, self.xBias, lengths)
         return z, zT.unsqueeze(1).unsqueeze(1)
 
     def extra_repr(self):

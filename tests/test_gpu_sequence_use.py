@@ -395,3 +395,32 @@ def test_a_student_of_padded_entries(tmp_path):
                 pr, qr = lp[r, rest].exp().sum(), lq[r, rest].exp().sum()
                 want += float(pr * (pr / qr).log())
     assert abs(losses[0][0] - want / 16) < 1e-4
+
+
+@pytest.mark.parametrize("gate", ["element", "node"])
+def test_what_padded_steps_of_a_layer_hold_does_not_matter(gate):
+    """Padding of NaN and inf gives the states and the gradients of zero padding, bit for bit: the filters never see it."""
+    torch.manual_seed(0)
+    B, T, F, N, H = 3, 20, 3, 30, 8
+    layer = gml.LinearHiddenState(F, H, 3, gate=gate)
+    layer.addGSO(torch.tensor(gso(N)))
+    layer.cuda()
+    lengths = torch.tensor([T, 7, 0], dtype=torch.int32, device="cuda")
+    dead = (torch.arange(T, device="cuda")[None, :] >= lengths[:, None])[:, :, None, None]
+    x, z0 = torch.randn(B, T, F, N, device="cuda"), torch.randn(B, H, N, device="cuda")
+    w, wT = torch.randn(B, T, H, N, device="cuda"), torch.randn(B, 1, 1, H, N, device="cuda")
+    a, S = torch.randn(H, 1, 2, F, device="cuda", requires_grad=True), layer._gso
+    f = torch.rand(B, T, 1, N, device="cuda")
+
+    def passes(padding):
+        leaf = torch.where(dead, padding, x).requires_grad_()
+        z, zT = layer(leaf, z0, lengths)
+        grads = torch.autograd.grad([z, zT], [leaf, *layer.parameters()], [w, wT])
+        y, yT = gml.LinearGRNN(a, S, leaf, z0, torch.tanh, None, f, lengths=lengths)
+        return [z, zT, *grads, y, yT, *torch.autograd.grad([y, yT], [leaf, a], [w, wT[:, 0, 0]])]
+    want = passes(torch.zeros_like(x))
+    bad = torch.full_like(x, float("nan"))
+    bad[:, ::2] = float("inf")
+    assert all(torch.isfinite(t).all() for t in want)
+    for i, (p, q) in enumerate(zip(passes(bad), want)):
+        assert torch.equal(p, q), i
