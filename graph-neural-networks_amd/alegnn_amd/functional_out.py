@@ -86,7 +86,8 @@ def distill_top(logits, indices, values, temperature=1.0, tail=False, dim=-1):
                   loss = sum_k p_k (log p_k - log q[i_k]).
       tail=True:  values are log probabilities (at this temperature), p_k = exp(values_k), and what is left to one is one more outcome:
                   loss = sum_k p_k (log p_k - log q[i_k]) + p_r (log p_r - log q_r), q_r = the mass of the outputs that are not named.
-                  (With every output named there are none: the loss is inf if the values leave any mass.)
+                  (With every output named there are none, and the loss is inf if the values leave any mass, be it by rounding: then take
+                  tail=False with values * temperature, which scales them to one.)
     A row without entries (tail=False: without mass) has loss 0 and gradient 0; an index that is named twice counts as two entries.  No factor
     temperature^2 is applied.  Differentiable (once, in reverse mode) in logits; the teacher's values are constants."""
     host = _lib.host()

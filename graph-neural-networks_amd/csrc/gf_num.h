@@ -23,11 +23,6 @@ template <> __device__ __forceinline__ gf_f16 gf_from_f<gf_f16>(float x) { retur
 
 template <typename D, int V> struct alignas(sizeof(D) * V) gf_vec { D e[V]; };
 
-template <typename D, int V> __device__ __forceinline__ void gf_load(const D* __restrict__ p, float (&out)[V]) {
-    const gf_vec<D, V> r = *reinterpret_cast<const gf_vec<D, V>*>(p);
-#pragma unroll
-    for (int i = 0; i < V; ++i) out[i] = gf_to_f<D>(r.e[i]);
-}
 template <typename D, int V> __device__ __forceinline__ void gf_store(D* __restrict__ p, const float (&v)[V]) {
     gf_vec<D, V> r;
 #pragma unroll

@@ -311,7 +311,7 @@ int gf_token_logp_backward(const void* logits, int64_t row_stride, const int64_t
  *   tail = 1: values are log probabilities, p_k = exp(values_k), what is left to one is one further outcome "none of these":
  *             loss = sum_k p_k (log p_k - log q[i_k]) + p_r (log p_r - log q_r),  q_r = sum of q over the outputs not named
  * A row without entries has loss 0 and gradient 0; an index named twice counts as two entries.  1 <= K <= 64.
- * stats [R, 3] and probs [R, K] fp32: what the backward pass needs. */
+ * stats [R, 3] and probs [R, K] fp32: what the backward pass needs (`tail` is in them: its argument there is not read). */
 size_t gf_distill_top_workspace_bytes(int64_t R, int32_t V, int32_t K, int32_t dtype);
 int gf_distill_top_forward(const void* logits, int64_t row_stride, const int64_t* indices, const float* values, float temperature, int32_t tail,
                            float* loss, float* stats, float* probs, void* workspace, size_t workspace_bytes, int32_t dtype, int64_t R, int32_t V,
