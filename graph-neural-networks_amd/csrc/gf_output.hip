@@ -12,8 +12,8 @@
 // Backward: one more read of the logits and one write; the few outputs that are named (token, alternatives, teacher's entries) are then
 // written over by the same workgroup.
 // Bound by HBM; for 16-bit logits the exponential (a quarter-rate instruction) and the conversions weigh about as much.  Reached: forward over
-// 2048 x 100k bf16 102 us (4.0 TB/s), with entropy and 8 alternatives over 4096 x 50001 118-125 us (3.4); gradients 131-144 us (5.7-6.3 TB/s read
-// and written; a copy of 4 GiB 4.7, of 128 MiB 7.2); 2000 x 10k fp32: 16 + 26 us; 1M rows of 5: 43 us with 3 alternatives.
+// 2048 x 100k bf16 104 + 8 us (tiles, join; 3.9 TB/s in the tiles), with entropy and 8 alternatives over 4096 x 50001 117 + 14 us (3.5); gradients
+// 131-139 us (5.9-6.2 TB/s read and written; a copy of 4 GiB 4.7, of 128 MiB 7.2); 2000 x 10k fp32: 16 + 4 and 26 us; 1M rows of 5: 43 us with 3 alternatives.
 // exp2_fast gives zero below 2^-126: a probability is off by less than that.
 // Sums are fp32 and in a fixed order; the K-wide part of the distillation loss is fp64 (a small difference of masses near one).
 #include "gf_num.h"
@@ -25,8 +25,8 @@ namespace {
 constexpr int kThr = 256;
 constexpr int kTopMax = 64;
 constexpr int kPackMax = 64;       // rows of up to so many outputs are packed into waves
-constexpr int kMaxNV = 4;          // 16-byte groups per thread and tile.  8 (twice the registers, a 64-bit hit mask) and 2 lost when the alternatives were
-                                   // still collected element by element: 189 and 177 us against 162 us for 4096 x 50001 bf16 with 8 of them
+constexpr int kMaxNV = 4;          // 16-byte groups per thread and tile: 4 / 2: 117 / 155 us for 4096 x 50001 bf16 with 8 alternatives, 104 / 103 without (8 would
+                                   // need a 64-bit hit mask; timed before there was one at all: 189 against 162 us)
 constexpr int kCand = 1024;        // candidates that are ranked in LDS; more (heavy ties) take the extraction loop
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -160,6 +160,9 @@ __device__ __forceinline__ void answer_top(const TokenOut& o, int64_t at, u64 ke
 // not fit).  The tile is read again, so that the usual case keeps no registers for this.
 // (4096 x 50001 bf16 but for 20 outputs ruled out, 8 / 64 alternatives: 984 / 4971 us with the extraction loop below alone,
 // 531 / 550 us with this; 134 / 197 us without the mask.)
+// Not for rows that rise or fall with the index: a full tile's threshold is the smallest of the waves' (k / 4)-th maxima, the wave with the low
+// values decides it, 1500-1800 of 8192 values pass, above the exact threshold too, and the loop is taken (4096 x 50001 bf16 sorted, 8 / 64
+// alternatives: 0.82 / 4.9 ms; values that fall as a power law of the index 0.21 / 0.40 ms).
 template <typename D, int NV>
 __device__ __forceinline__ int collect_ties(const Row<D>& row, int64_t g0, float tm, bool full, int top, unsigned* s_thr, int* s_n, u64* s_cand) {
     constexpr int VE = Row<D>::VE;

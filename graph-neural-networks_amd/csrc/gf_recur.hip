@@ -23,14 +23,18 @@
 
 namespace {
 
-// Chosen by measurement (GPU time; the figures of a choice are from one build, later steps made both sides faster):
-constexpr int kL = 4;              // steps per thread and slab.  8 need twice the registers: backward of 32 x 257 x 53824 bf16 1.32 / 1.69 ms, 65537 x 808 301 / 416 us
-constexpr int kGW = 4;             // time groups of a wave: 4 against 8: 0.89 / 1.02 ms, against 2 with 8 steps each: 0.89 / 0.97 ms (the same backward)
-constexpr int kMaxSplit = 128;     // splits of a long time axis: 128 / 64 / 256: 307 / 344 / 323 us for 65537 x 808 bf16, forward and backward
+// Chosen by measurement (GPU time, forward and backward):
+constexpr int kL = 4;              // steps per thread and slab: 4 / 8: 1.37 / 1.52 ms for 32 x 257 x 53824 bf16 (twice the registers), 221 / 208 us for 65537 x 808
+constexpr int kGW = 4;             // time groups of a wave.  Timed before the joins by row swaps, which are for 4: backward of 32 x 257 x 53824 with 4 / 8 / 2
+                                   // (of 8 steps each) 0.89 / 1.02 / 0.97 ms
+constexpr int kMaxSplit = 128;     // splits of a long time axis: 64 / 128 / 256: 238 / 221 / 210 us for 65537 x 808 bf16 (on an earlier form 344 / 307 / 323)
 
 // What the kernels reach now: 32 x 257 x 53824 bf16 with lengths 0 .. 257: forward 0.47 ms, backward 0.90 ms = 4.9 TB/s of the rows they touch (a large
-// copy: 4.7); 65537 x 808 bf16 with a gate per step: split 21 + forward 49, split 33 + backward 110 us: the instructions per element (30 forward,
+// copy: 4.7); 65537 x 808 bf16 with a gate per step: split 20 + forward 50, split 33 + backward 111 us: the instructions per element (30 forward,
 // 50 backward in a join of 16 steps) weigh as much as the bytes there; 20 x 100 x 1600 fp32: forward 11, backward 20, gate sums 6 us.
+// What costs more than its bytes: gates that lack one of the channel axes (their products go through memory in fp32: 32 x 257 x 32 x 1682 bf16 with two
+// node / feature gates: forward 0.77 / 0.57, backward 1.75 / 1.46, sums 0.73 / 1.29 ms, full gates 0.70 + 1.25), and odd channel counts (one channel
+// per thread: 32 x 257 x 31 x 1681 with full gates 1.46 + 2.76 ms in bf16, 2.09 + 4.27 in fp32, against 1.42 + 2.49 for 32 x 1682 in fp32).
 struct Gate {                      // a gate of shape [B|1, T, H|1, N|1]: element (b, t, h, n) at b sb + t st + channel offset
     const void* p;
     int64_t sb;
