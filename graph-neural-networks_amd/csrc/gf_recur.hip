@@ -681,8 +681,9 @@ __global__ __launch_bounds__(64 * (WT == 1 ? 4 : WT)) void recur_bwd_kernel(cons
 
 // Sum of the fp32 products [rows, T, inner, H, N] ... over the axes a gate does not have, in a fixed order: out[b, t, h, n] (gate shape).
 // src [nb, B, T, Hs, Ns] : nb partial rows; axes: nb always, B if !GF_GATE_B, Hs if !(kind & H), Ns if !(kind & N).
-// One wave per output element where the node axis is summed, one thread per element otherwise (coalesced over nodes).
-__device__ __forceinline__ float sum_strided(const float* __restrict__ p, int n, int64_t stride, float s) {   // in order, eight loads in flight
+// One wave per output element where the node axis is summed, one thread per element otherwise (coalesced over nodes).  The sums are fp64 and rounded
+// once: a gate per step of an odd number of channels has thousands of partial ones (one after the other in fp32 they were off by 6e-7 of the result).
+__device__ __forceinline__ double sum_strided(const float* __restrict__ p, int n, int64_t stride, double s) {   // in order, eight loads in flight
     int i = 0;
     for (; i + 8 <= n; i += 8) {
         float v[8];
@@ -722,14 +723,14 @@ __global__ __launch_bounds__(256) void recur_fold_kernel(Fold f0, Fold f1, int B
         const int t = (int)(o2 % T), b = (int)(o2 / T);
         const float* p = src + ((int64_t)b * T + t) * row + (int64_t)h * Ns + n;
         const int hs = Ho == 1 ? Hs : 1, bs = Bo == 1 ? B : 1;
-        float s = 0.f;
+        double s = 0.0;
         if (byN) {
             for (int k = 0; k < nb * bs; ++k)                   // (nb > 1 only with Hs = Ns = 1)
                 for (int hh = 0; hh < hs; ++hh)
                     for (int m = lane; m < Ns; m += 64) s += p[(int64_t)k * T * row + (int64_t)hh * Ns + m];
 #pragma unroll
             for (int off = 1; off < 64; off <<= 1) s += __shfl_xor(s, off);
-            if (lane == 0) out[o] = gf_from_f<D>(s);
+            if (lane == 0) out[o] = gf_from_f<D>((float)s);
         } else {
             if (hs > 1) {
                 for (int bb = 0; bb < bs; ++bb) s = sum_strided(p + (int64_t)bb * T * row, hs, Ns, s);
@@ -738,7 +739,7 @@ __global__ __launch_bounds__(256) void recur_fold_kernel(Fold f0, Fold f1, int B
             } else {
                 s = sum_strided(p, nb, (int64_t)B * T * row, s);
             }
-            out[o] = gf_from_f<D>(s);
+            out[o] = gf_from_f<D>((float)s);
         }
     }
 }

@@ -329,3 +329,19 @@ def test_many_channels_and_unlike_lengths(kc, kh, dtype):
     ins = make(B, T, H, N, kc, kh, DT[dtype], seed=21)
     lengths = torch.tensor([0, 1, 15, 16, 17, 31, 32, 33, 48, 50, 63, 64, 65, 69, 70, 70], dtype=torch.int32)
     check(run(*ins[:4], lengths, *ins[4:]), ins, lengths, DT[dtype])
+
+
+@pytest.mark.parametrize("shape", [(3, 1, 29, 701), (2, 7, 31, 513), (2, 40, 17, 333), (1, 700, 3, 401), (40, 3, 2, 700)], ids=str)
+@pytest.mark.parametrize("kind", ["time", "time1", "node", "node1", "feature", "full1"])
+def test_gate_sums_are_rounded_once(shape, kind):
+    """With q_check = 0 and q_hat = 1 the gates' gradients are sums of dz_t u_{t-1} and dz_t u_t: whole numbers here, each product below 2^16 and each
+    wave's sum of at most 256 of them exact in float32.  What is left is the sum of the partial ones: rounded once, it is the exact sum's float32."""
+    B, T, H, N = shape
+    g = torch.Generator().manual_seed(sum(shape))
+    u, dz = (torch.randint(0, 256, (B, T, H, N), generator=g).float() for _ in range(2))
+    z0 = torch.randint(0, 256, (B, H, N), generator=g).float()
+    gate = gate_shape(kind, B, T, H, N)
+    out = run(u, torch.zeros(gate), torch.ones(gate), z0, None, dz, torch.zeros(B, H, N))
+    prev = np.concatenate((f64(z0)[:, None], f64(u)[:, :-1]), 1)
+    for k, p in (("dq_check", f64(dz) * prev), ("dq_hat", f64(dz) * f64(u))):
+        assert np.array_equal(out[k], ref.fold(p, gate).astype(np.float32).astype(np.float64)), k
