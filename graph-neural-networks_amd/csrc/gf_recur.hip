@@ -15,7 +15,7 @@
 // fp32 checkpoint per slab instead of being read back rounded.  Bound by HBM: forward reads u, qc, qh and writes z, backward reads u, qc,
 // qh, dz and writes du, dqc, dqh.
 //
-// State, products and sums are fp32; outputs are rounded once.  Steps at or behind a sequence's length leave the state as it is (A = 1,
+// State and products are fp32, the gate sums over a launch's partial ones fp64; outputs are rounded once.  Steps at or behind a sequence's length leave the state as it is (A = 1,
 // h = 0), whatever they hold (their values are replaced behind the load), and their outputs and gradients are zero.
 #include "gf_num.h"
 
