@@ -490,7 +490,7 @@ class HiddenState(nn.Module):
 
 def _live_steps(x, lengths):
     """x [B,T,F,N] with zeros in the steps that do not count: a filter would carry what they hold (NaN, inf) into its taps' gradient."""
-    if lengths is None:
+    if lengths is None or lengths.shape != x.shape[:1] or lengths.device != x.device:       # (linear_recurrence says what is wrong with them)
         return x
     live = torch.arange(x.shape[1], device=x.device) < lengths[:, None]
     return torch.where(live[:, :, None, None], x, 0.0)

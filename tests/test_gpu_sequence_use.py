@@ -424,3 +424,18 @@ def test_what_padded_steps_of_a_layer_hold_does_not_matter(gate):
     assert all(torch.isfinite(t).all() for t in want)
     for i, (p, q) in enumerate(zip(passes(bad), want)):
         assert torch.equal(p, q), i
+
+
+def test_lengths_of_a_layer_are_refused_as_the_recurrences_own():
+    layer = gml.LinearHiddenState(2, 4, 2)
+    layer.addGSO(torch.tensor(gso(30)))
+    layer.cuda()
+    x = torch.randn(3, 5, 2, 30, device="cuda")
+    for lengths, kind, word in ((torch.zeros(2, dtype=torch.int32, device="cuda"), AssertionError, "lengths"),
+                                (torch.zeros(3, 1, dtype=torch.int32, device="cuda"), AssertionError, "lengths"),
+                                (torch.zeros(3, dtype=torch.int64, device="cuda"), TypeError, "lengths"),
+                                (torch.zeros(3, dtype=torch.int32), RuntimeError, "no CPU fallback")):
+        with pytest.raises(kind, match=word):
+            layer(x, None, lengths)
+        with pytest.raises(kind, match=word):
+            gml.LinearGRNN(layer.aWeights, layer._gso, x, None, None, None, torch.ones(3, 5, 1, 1, device="cuda"), lengths=lengths)
